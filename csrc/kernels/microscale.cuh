@@ -1,0 +1,200 @@
+// Microscaled number formats: a block of consecutive elements of a row shares one scale byte.
+//
+//   mxfp4  e2m1 elements (largest 6), 32 per scale, scale = a power of two (e8m0)
+//   nvfp4  e2m1 elements, 16 per scale, scale = e4m3, times one fp32 scale g of the whole tensor
+//   mxfp8  e4m3 elements (largest 448), 32 per scale, scale = a power of two (e8m0)
+//
+// Codes: 4-bit elements two to a byte, the even element in the low half; rows padded to 16 bytes.
+// Scales: tiles of 128 rows x 4 blocks (512 bytes), byte [r / 128][b / 4][r % 32][(r / 32) % 4][b % 4]
+// for row r, block b, so that one tile is the 32 x 16 byte matrix that tcgen05.cp spreads over
+// the 32 lanes of tensor memory; rows and blocks past the end are zero bytes.
+#pragma once
+
+#include <cuda_fp4.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+#include "microscale.h"
+
+namespace mmltk {
+namespace mx {
+
+template <MxFormat F>
+struct Traits;
+template <>
+struct Traits<MxFormat::kMxFp4> {
+    static constexpr int kBlock = 32, kBits = 4;
+    static constexpr bool kPow2 = true;
+};
+template <>
+struct Traits<MxFormat::kNvFp4> {
+    static constexpr int kBlock = 16, kBits = 4;
+    static constexpr bool kPow2 = false;
+};
+template <>
+struct Traits<MxFormat::kMxFp8> {
+    static constexpr int kBlock = 32, kBits = 8;
+    static constexpr bool kPow2 = true;
+};
+
+// Offset of the scale byte of row r, block b in the tiled layout with kt = ceil(blocks / 4) tiles along a row.
+__device__ __forceinline__ int64_t scale_offset(int64_t r, int b, int kt) {
+    return ((r >> 7) * kt + (b >> 2)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (b & 3);
+}
+
+struct BlockScale {
+    uint32_t byte;   // the stored scale
+    float inv;       // what x is multiplied with before it is rounded to an element
+};
+
+// Power-of-two scale: the smallest 2^p whose 2^p * (largest element) is not below amax, so no element
+// saturates.  amax = 1.M * 2^(E - 127) against 1.5 * 2^2 (e2m1) or 1.75 * 2^8 (e4m3), on the bits;
+// clamped at 2^-127.  A block with an infinity or NaN gets the NaN scale (0xff): its values read back NaN
+// whatever their codes (zero for its finite elements and its padding).
+template <int kBits>
+__device__ __forceinline__ BlockScale pow2_scale(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    BlockScale s;
+    if (u >= 0x7f800000u) {
+        s.byte = 0xff;
+        s.inv = 0.f;
+        return s;
+    }
+    const int e = static_cast<int>(u >> 23), m = static_cast<int>(u & 0x7fffffu);
+    const int p = kBits == 4 ? e - 2 + (m > 0x400000) : e - 8 + (m > 0x600000);
+    s.byte = static_cast<uint32_t>(max(p, 0));
+    s.inv = __uint_as_float((254u - s.byte) << 23);   // 2^-(byte - 127): byte <= 253, a normal number
+    return s;
+}
+
+// e4m3 scale of amax / 6 on the tensor scale's grid; the elements are x times the rounded reciprocal
+// 1 / (s g) (one division per block instead of one per element).  s = 0 (amax below 2^-10 * 6 g): all zero.
+__device__ __forceinline__ BlockScale e4m3_scale(float amax, float g) {
+    BlockScale s;
+    if (__float_as_uint(amax) >= 0x7f800000u) {
+        s.byte = 0x7f;
+        s.inv = 0.f;
+        return s;
+    }
+    const float t = fminf(amax / (6.0f * g), 448.0f);
+    const __nv_fp8_storage_t q = __nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3);
+    s.byte = q;
+    const float v = __half2float(__half(__nv_cvt_fp8_to_halfraw(q, __NV_E4M3)));
+    s.inv = v > 0.f ? 1.0f / (v * g) : 0.f;
+    return s;
+}
+
+template <MxFormat F>
+__device__ __forceinline__ BlockScale block_scale(float amax, float g) {
+    if constexpr (Traits<F>::kPow2) {
+        return pow2_scale<Traits<F>::kBits>(amax);
+    } else {
+        return e4m3_scale(amax, g);
+    }
+}
+
+// max that keeps a NaN (fmaxf drops it): on the bits of |x|, where NaN > infinity > every number
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+__device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint32_t cvt_e2m1x2(float lo, float hi) {
+    return __nv_cvt_float2_to_fp4x2(make_float2(lo, hi), __NV_E2M1, cudaRoundNearest);
+}
+__device__ __forceinline__ uint32_t cvt_e4m3x4(const float* v, float inv) {
+    return cvt_e4m3x2(v[0] * inv, v[1] * inv) | (cvt_e4m3x2(v[2] * inv, v[3] * inv) << 16);
+}
+__device__ __forceinline__ uint32_t cvt_e2m1x8(const float* v, float inv) {
+    return cvt_e2m1x2(v[0] * inv, v[1] * inv) | (cvt_e2m1x2(v[2] * inv, v[3] * inv) << 8) |
+           (cvt_e2m1x2(v[4] * inv, v[5] * inv) << 16) | (cvt_e2m1x2(v[6] * inv, v[7] * inv) << 24);
+}
+
+__device__ __forceinline__ float2 e4m3x2_to_f(uint32_t w) {
+    return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w), __NV_E4M3)));
+}
+__device__ __forceinline__ float2 e2m1x2_to_f(uint32_t w) {
+    return __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(w), __NV_E2M1)));
+}
+
+// Value of a stored scale byte.
+template <MxFormat F>
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+    if constexpr (Traits<F>::kPow2) {
+        if (byte == 0xff) return __uint_as_float(0x7fc00000u);
+        return byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);   // 0: 2^-127, a subnormal
+    } else {
+        return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
+    }
+}
+
+// Scale of a whole tensor (nvfp4) from its largest magnitude: puts the largest block scale at 448.
+// 2^-100 keeps 1 / (s g) finite; a tensor without a finite maximum keeps g = 1.
+__device__ __forceinline__ float tensor_scale(uint32_t amax_bits) {
+    const float a = __uint_as_float(amax_bits);
+    if (amax_bits == 0 || amax_bits >= 0x7f800000u) return 1.0f;
+    return fmaxf(a / 2688.0f, 7.888609052210118e-31f);
+}
+
+// ---------------------------------------------------------------- 16-byte vectors of the three input types
+template <typename T>
+struct VecOf {
+    static constexpr int kN = 16 / sizeof(T);
+};
+__device__ __forceinline__ void unpack16(const uint4& w, float* f, __nv_bfloat16) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(u[i] << 16);
+        f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void unpack16(const uint4& w, float* f, __half) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        f[2 * i] = t.x;
+        f[2 * i + 1] = t.y;
+    }
+}
+__device__ __forceinline__ void unpack16(const uint4& w, float* f, float) {
+    f[0] = __uint_as_float(w.x);
+    f[1] = __uint_as_float(w.y);
+    f[2] = __uint_as_float(w.z);
+    f[3] = __uint_as_float(w.w);
+}
+__device__ __forceinline__ uint4 pack16(const float* f, __nv_bfloat16) {
+    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                      pack_bf16x2(f[6], f[7]));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint4 pack16(const float* f, __half) {
+    return make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]),
+                      pack_f16x2(f[6], f[7]));
+}
+__device__ __forceinline__ uint4 pack16(const float* f, float) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+
+}  // namespace mx
+}  // namespace mmltk
+
+// element type dispatch of the microscale / RMS-norm kernels (bf16, f16, fp32)
+#define MMLTK_DISPATCH_ELT(et, ...)                    \
+    [&]() -> cudaError_t {                             \
+        if ((et) == ::mmltk::Elt::kBF16) {             \
+            using elt_t = __nv_bfloat16;               \
+            return __VA_ARGS__();                      \
+        } else if ((et) == ::mmltk::Elt::kF16) {       \
+            using elt_t = __half;                      \
+            return __VA_ARGS__();                      \
+        } else if ((et) == ::mmltk::Elt::kF32) {       \
+            using elt_t = float;                       \
+            return __VA_ARGS__();                      \
+        }                                              \
+        return cudaErrorInvalidValue;                  \
+    }()

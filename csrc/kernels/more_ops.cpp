@@ -278,6 +278,7 @@ void register_more_ops(pybind11::module& m) {
     register_image_ops(m);
     register_attn_ops(m);
     register_overlay_ops(m);
+    register_mx_ops(m);
     register_debug_ops(m);
 }
 

@@ -1,0 +1,408 @@
+// Root-mean-square norm over the last dimension, with the residual's addition, and its backward.
+//
+//   h = round(x + r),  rstd = (mean(h^2) + eps)^-1/2,  y = h rstd w
+//   gx = gr = gh + rstd w gy - h rstd^3 mean(h w gy),   gw = sum_rows gy h rstd
+//
+// y goes out in x's type, or quantised (microscale.cuh) straight from its fp32 values, with the
+// scales in the tiled layout that the tensor-core product reads.
+//
+// Memory-bound.  A row is held in registers by a group of threads -- a warp up to 1024 16-bit
+// elements, a CTA of 128 to 512 threads beyond -- so every element is read once; statistics are
+// fp32.  A thread's elements are 16-byte vectors kGroup vectors apart (VEC = 1 where the width,
+// the pitch or an address is not a multiple of 16 bytes), so the 4 or 8 threads of a scale block
+// are neighbours in a warp and find its maximum with two or three shuffles.
+#include "microscale.cuh"
+
+namespace mmltk {
+
+namespace {
+
+using namespace mx;
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float* f) {
+    if constexpr (VEC == 1) {
+        f[0] = to_f(*p);
+    } else {
+        unpack16(*reinterpret_cast<const uint4*>(p), f, T());
+    }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float* f) {
+    if constexpr (VEC == 1) {
+        *p = from_f<T>(f[0]);
+    } else {
+        *reinterpret_cast<uint4*>(p) = pack16(f, T());
+    }
+}
+// weights: x's type or fp32
+template <typename T, int VEC>
+__device__ __forceinline__ void load_w(const void* w, bool f32, int i, float* f) {
+    if (f32) {
+        const float* p = static_cast<const float*>(w) + i;
+#pragma unroll
+        for (int e = 0; e < VEC; e += (VEC >= 4 ? 4 : 1)) {
+            if constexpr (VEC >= 4) {
+                const float4 t = *reinterpret_cast<const float4*>(p + e);
+                f[e] = t.x; f[e + 1] = t.y; f[e + 2] = t.z; f[e + 3] = t.w;
+            } else {
+                f[e] = p[e];
+            }
+        }
+    } else {
+        load_vec<T, VEC>(static_cast<const T*>(w) + i, f);
+    }
+}
+
+// Sum over the kGroup threads of a row, the same value (and order) in all of them.
+template <int kGroup>
+__device__ __forceinline__ float group_sum(float s, float* red) {
+    s = warp_sum(s);
+    if constexpr (kGroup > 32) {
+        constexpr int kWarps = kGroup / 32;
+        const int lane = threadIdx.x & 31;
+        if (lane == 0) red[threadIdx.x >> 5] = s;
+        __syncthreads();
+        s = warp_sum(lane < kWarps ? red[lane] : 0.f);
+    }
+    return s;
+}
+
+// Quantises the VEC values at column i of row r (a whole warp calls; i < span), stores codes and scales.
+template <MxFormat F, int VEC>
+__device__ __forceinline__ void quantize_store(const float* v, int i, int64_t r, int64_t pitch, int kt, int span,
+                                               uint8_t* codes, uint8_t* scales, float g) {
+    using Tr = Traits<F>;
+    constexpr int kThreads = Tr::kBlock / VEC;      // threads of a block: 32 / 16, 8 / 4 or 4 / 2
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) m = max(m, abs_bits(v[e]));
+#pragma unroll
+    for (int o = 1; o < kThreads; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const BlockScale sc = block_scale<F>(__uint_as_float(m), g);
+    const int lane = threadIdx.x & 31;
+    uint8_t* row = codes + r * pitch;
+    if constexpr (Tr::kBits == 8) {
+        if (i < pitch) {
+            if constexpr (VEC == 8) {
+                *reinterpret_cast<uint2*>(row + i) = make_uint2(cvt_e4m3x4(v, sc.inv), cvt_e4m3x4(v + 4, sc.inv));
+            } else if constexpr (VEC == 4) {
+                *reinterpret_cast<uint32_t*>(row + i) = cvt_e4m3x4(v, sc.inv);
+            } else {
+                row[i] = static_cast<uint8_t>(cvt_e4m3x2(v[0] * sc.inv, 0.f));
+            }
+        }
+    } else {
+        if constexpr (VEC == 1) {
+            const float hi = __shfl_down_sync(0xffffffffu, v[0], 1);
+            if (i < 2 * pitch && (lane & 1) == 0) row[i >> 1] = static_cast<uint8_t>(cvt_e2m1x2(v[0] * sc.inv, hi * sc.inv));
+        } else if (i < 2 * pitch) {
+            if constexpr (VEC == 8) {
+                *reinterpret_cast<uint32_t*>(row + (i >> 1)) = cvt_e2m1x8(v, sc.inv);
+            } else {
+                *reinterpret_cast<uint16_t*>(row + (i >> 1)) = static_cast<uint16_t>(
+                    cvt_e2m1x2(v[0] * sc.inv, v[1] * sc.inv) | (cvt_e2m1x2(v[2] * sc.inv, v[3] * sc.inv) << 8));
+            }
+        }
+    }
+    // the four scales of a tile's row, one 4-byte store, where a warp holds all four
+    if constexpr (4 * kThreads <= 32) {
+        uint32_t b = sc.byte;
+        b |= __shfl_down_sync(0xffffffffu, b, kThreads) << 8;
+        b |= __shfl_down_sync(0xffffffffu, b, 2 * kThreads) << 16;
+        if (i < span && (lane & (4 * kThreads - 1)) == 0)
+            *reinterpret_cast<uint32_t*>(scales + scale_offset(r, i / Tr::kBlock, kt)) = b;
+    } else {
+        if (i < span && (lane & (kThreads - 1)) == 0)
+            scales[scale_offset(r, i / Tr::kBlock, kt)] = static_cast<uint8_t>(sc.byte);
+    }
+}
+
+template <typename T, int VEC, int kGroup, int KV, bool kQuant>
+__global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(RmsFwdArgs a) {
+    __shared__ float red[32];
+    constexpr int kRows = kGroup == 32 ? 8 : 1;
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + (kGroup == 32 ? threadIdx.x >> 5 : 0);
+    const int t = threadIdx.x & (kGroup - 1);
+    const int kt = kQuant ? static_cast<int>(mx_scale_tiles(a.fmt, a.dim)) : 0;
+    if (r >= a.rows) {   // (all of the row's threads) rows that fill the last scale tile: zero scales
+        if (kQuant && r < (a.rows + 127) / 128 * 128)
+            for (int i = t; i < kt; i += kGroup)
+                *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.scales) + scale_offset(r, 4 * i, kt)) = 0;
+        return;
+    }
+    const T* xr = static_cast<const T*>(a.x) + r * a.ldx;
+    const T* rr = a.res ? static_cast<const T*>(a.res) + r * a.ldr : nullptr;
+    float v[KV][VEC];
+#pragma unroll
+    for (int k = 0; k < KV; ++k) {
+        const int i = (k * kGroup + t) * VEC;
+        if (i < a.dim) {
+            load_vec<T, VEC>(xr + i, v[k]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[k][e] = 0.f;
+        }
+    }
+    if (rr) {
+        T* hr = static_cast<T*>(a.h) + r * a.dim;
+        float u[KV][VEC];
+#pragma unroll
+        for (int k = 0; k < KV; ++k) {
+            const int i = (k * kGroup + t) * VEC;
+            if (i < a.dim) load_vec<T, VEC>(rr + i, u[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < KV; ++k) {
+            const int i = (k * kGroup + t) * VEC;
+            if (i < a.dim) {
+                // the norm sees the sum as it is stored, so that its backward can start from h
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[k][e] = to_f(from_f<T>(v[k][e] + u[k][e]));
+                store_vec<T, VEC>(hr + i, v[k]);
+            }
+        }
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < KV; ++k)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s = fmaf(v[k][e], v[k][e], s);
+    s = group_sum<kGroup>(s, red);
+    const float rstd = 1.f / sqrtf(s / static_cast<float>(a.dim) + a.eps);
+    if (a.rstd && t == 0) a.rstd[r] = rstd;
+    const int span = kQuant ? kt * 4 * mx_block(a.fmt) : a.dim;
+    float g = 1.f;
+    if (kQuant && a.g) g = *a.g;
+#pragma unroll
+    for (int k = 0; k < KV; ++k) {
+        const int i = (k * kGroup + t) * VEC;
+        if (i < a.dim) {
+            float w[VEC];
+            load_w<T, VEC>(a.w, a.w_f32, i, w);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[k][e] = v[k][e] * rstd * w[e];
+            if constexpr (!kQuant) store_vec<T, VEC>(static_cast<T*>(a.y) + r * a.dim + i, v[k]);
+        }
+        if constexpr (kQuant) {
+            if ((k * kGroup + (t & ~31)) * VEC >= span) continue;     // warp-uniform
+            uint8_t* codes = static_cast<uint8_t*>(a.codes);
+            uint8_t* scales = static_cast<uint8_t*>(a.scales);
+            const int64_t pitch = mx_pitch(a.fmt, a.dim);
+            if (a.fmt == MxFormat::kMxFp8)
+                quantize_store<MxFormat::kMxFp8, VEC>(v[k], i, r, pitch, kt, span, codes, scales, g);
+            else if (a.fmt == MxFormat::kMxFp4)
+                quantize_store<MxFormat::kMxFp4, VEC>(v[k], i, r, pitch, kt, span, codes, scales, g);
+            else
+                quantize_store<MxFormat::kNvFp4, VEC>(v[k], i, r, pitch, kt, span, codes, scales, g);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- backward
+// Persistent: a group of threads walks rows and keeps its columns' part of gw in registers; one partial
+// row per CTA, summed in a fixed order by rms_gw_kernel (no atomics: the same bits every run).
+template <typename T, int VEC, int kGroup, int KV>
+__global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_bwd_kernel(RmsBwdArgs a) {
+    constexpr int kRows = kGroup == 32 ? 8 : 1;
+    __shared__ float red[2][32];
+    __shared__ float part[kGroup == 32 ? 8 * 32 * VEC : 1];
+    const int sub = kGroup == 32 ? threadIdx.x >> 5 : 0;
+    const int t = threadIdx.x & (kGroup - 1);
+    float acc[KV][VEC];
+#pragma unroll
+    for (int k = 0; k < KV; ++k)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[k][e] = 0.f;
+    const float inv_dim = 1.f / static_cast<float>(a.dim);
+    int turn = 0;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + sub; r < a.rows;
+         r += static_cast<int64_t>(gridDim.x) * kRows, turn ^= 1) {
+        const float rstd = a.rstd[r];
+        float hv[KV][VEC], gv[KV][VEC], ev[KV][VEC];
+#pragma unroll
+        for (int k = 0; k < KV; ++k) {
+            const int i = (k * kGroup + t) * VEC;
+            if (i < a.dim) {
+                load_vec<T, VEC>(static_cast<const T*>(a.h) + r * a.ldh + i, hv[k]);
+                if (a.gy) load_vec<T, VEC>(static_cast<const T*>(a.gy) + r * a.ldgy + i, gv[k]);
+                if (a.gh) load_vec<T, VEC>(static_cast<const T*>(a.gh) + r * a.ldgh + i, ev[k]);
+            }
+        }
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < KV; ++k) {
+            const int i = (k * kGroup + t) * VEC;
+            if (i < a.dim && a.gy) {
+                float w[VEC];
+                load_w<T, VEC>(a.w, a.w_f32, i, w);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    acc[k][e] = fmaf(gv[k][e], hv[k][e] * rstd, acc[k][e]);
+                    gv[k][e] *= w[e];
+                    s = fmaf(hv[k][e], gv[k][e], s);
+                }
+            }
+        }
+        s = group_sum<kGroup>(s, red[turn]);     // two turns: the next row's sums do not meet this row's readers
+        const float c = s * inv_dim * rstd * rstd * rstd;
+#pragma unroll
+        for (int k = 0; k < KV; ++k) {
+            const int i = (k * kGroup + t) * VEC;
+            if (i < a.dim) {
+                float o[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    o[e] = a.gy ? fmaf(rstd, gv[k][e], -c * hv[k][e]) : 0.f;
+                    if (a.gh) o[e] += ev[k][e];
+                }
+                store_vec<T, VEC>(static_cast<T*>(a.gx) + r * a.dim + i, o);
+            }
+        }
+    }
+    if (!a.partial) return;
+    float* dst = a.partial + static_cast<int64_t>(blockIdx.x) * a.dim;
+#pragma unroll
+    for (int k = 0; k < KV; ++k) {
+        const int i = (k * kGroup + t) * VEC;
+        if constexpr (kGroup == 32) {
+            // the eight warps' parts of these columns, added in the order of the warps
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) part[(sub * VEC + e) * 32 + t] = acc[k][e];
+            __syncthreads();
+            for (int j = threadIdx.x; j < 32 * VEC; j += 256) {
+                const int lane = j / VEC, e = j % VEC, col = (k * 32 + lane) * VEC + e;
+                float sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < 8; ++w) sum += part[(w * VEC + e) * 32 + lane];
+                if (col < a.dim) dst[col] = sum;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (i + e < a.dim) dst[i + e] = acc[k][e];
+        }
+    }
+}
+
+// gw[c] = sum of the partial rows; 32 columns a CTA, 8 threads a column
+template <typename T>
+__global__ void __launch_bounds__(256) rms_gw_kernel(const float* __restrict__ partial, int rows, int dim,
+                                                     void* __restrict__ gw, bool w_f32) {
+    __shared__ float red[8][33];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), y = threadIdx.x >> 5;
+    float s = 0.f;
+    if (c < dim) {
+#pragma unroll 8
+        for (int r = y; r < rows; r += 8) s += partial[static_cast<int64_t>(r) * dim + c];
+    }
+    red[y][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (y == 0 && c < dim) {
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += red[j][threadIdx.x];
+        if (w_f32) static_cast<float*>(gw)[c] = sum;
+        else static_cast<T*>(gw)[c] = from_f<T>(sum);
+    }
+}
+
+// Threads per row and vectors per thread: the smallest group that holds `elems` (a warp while a thread
+// keeps at most 4 vectors, i.e. 1024 16-bit elements).
+template <int VEC, typename Fn>
+cudaError_t by_width(int elems, Fn&& fn) {
+    auto go = [&](auto g, auto kv) { return fn(g, kv); };
+#define MMLTK_RMS_WIDTH(G, KV) \
+    if (elems <= G * KV * VEC) return go(std::integral_constant<int, G>{}, std::integral_constant<int, KV>{})
+    if constexpr (VEC == 1) {
+        MMLTK_RMS_WIDTH(128, 8);
+        MMLTK_RMS_WIDTH(256, 16);
+        MMLTK_RMS_WIDTH(512, 32);
+    } else {
+        MMLTK_RMS_WIDTH(32, 1);
+        MMLTK_RMS_WIDTH(32, 2);
+        MMLTK_RMS_WIDTH(32, 4);
+        MMLTK_RMS_WIDTH(128, 2);
+        MMLTK_RMS_WIDTH(128, 4);
+        MMLTK_RMS_WIDTH(256, 4);
+        MMLTK_RMS_WIDTH(512, 4);
+        if constexpr (VEC == 4) MMLTK_RMS_WIDTH(512, 8);
+    }
+#undef MMLTK_RMS_WIDTH
+    return cudaErrorInvalidValue;
+}
+
+bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+}  // namespace
+
+cudaError_t launch_rms_fwd(Elt et, const RmsFwdArgs& a, cudaStream_t st) {
+    if (a.rows <= 0) return cudaSuccess;
+    if (a.dim <= 0 || a.dim > kRmsMaxDim) return cudaErrorInvalidValue;
+    const bool quant = a.codes != nullptr;
+    const int elems = quant ? static_cast<int>(mx_scale_tiles(a.fmt, a.dim)) * 4 * mx_block(a.fmt) : a.dim;
+    const int64_t rows = quant ? (a.rows + 127) / 128 * 128 : a.rows;
+    return MMLTK_DISPATCH_ELT(et, [&]() -> cudaError_t {
+        using T = elt_t;
+        constexpr int kN = VecOf<T>::kN;
+        const bool vec = a.dim % kN == 0 && a.ldx % kN == 0 && aligned(a.x) && aligned(a.w) &&
+                         (!a.res || (a.ldr % kN == 0 && aligned(a.res)));
+        auto run = [&](auto vc) -> cudaError_t {
+            constexpr int VEC = decltype(vc)::value;
+            return by_width<VEC>(elems, [&](auto gc, auto kc) -> cudaError_t {
+                constexpr int G = decltype(gc)::value, KV = decltype(kc)::value;
+                const int64_t per = G == 32 ? 8 : 1, blocks = (rows + per - 1) / per;
+                if (blocks >= (int64_t(1) << 31)) return cudaErrorInvalidValue;
+                const int threads = G == 32 ? 256 : G;
+                if (quant)
+                    rms_fwd_kernel<T, VEC, G, KV, true><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
+                else
+                    rms_fwd_kernel<T, VEC, G, KV, false><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
+                return cudaGetLastError();
+            });
+        };
+        if (vec) return run(std::integral_constant<int, kN>{});
+        return run(std::integral_constant<int, 1>{});
+    });
+}
+
+namespace {
+// CTAs of the backward: two or more an SM at these register counts, fewer for few rows
+int bwd_blocks(int64_t rows, int dim, int group) {
+    const int64_t per = group == 32 ? 8 : 1;
+    const int per_sm = group == 32 ? 4 : (group >= 512 ? 2 : 4);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, num_sms() * per_sm)));
+}
+}  // namespace
+
+int rms_bwd_partials(Elt, int64_t rows, int) {
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, num_sms() * 4)));
+}
+
+cudaError_t launch_rms_bwd(Elt et, const RmsBwdArgs& a, cudaStream_t st) {
+    if (a.dim <= 0 || a.dim > kRmsMaxDim) return cudaErrorInvalidValue;
+    return MMLTK_DISPATCH_ELT(et, [&]() -> cudaError_t {
+        using T = elt_t;
+        constexpr int kN = VecOf<T>::kN;
+        const bool vec = a.dim % kN == 0 && aligned(a.h) && a.ldh % kN == 0 && aligned(a.w) &&
+                         (!a.gy || (a.ldgy % kN == 0 && aligned(a.gy))) &&
+                         (!a.gh || (a.ldgh % kN == 0 && aligned(a.gh)));
+        auto run = [&](auto vc) -> cudaError_t {
+            constexpr int VEC = decltype(vc)::value;
+            return by_width<VEC>(a.dim, [&](auto gc, auto kc) -> cudaError_t {
+                constexpr int G = decltype(gc)::value, KV = decltype(kc)::value;
+                const int blocks = bwd_blocks(a.rows, a.dim, G);
+                rms_bwd_kernel<T, VEC, G, KV><<<blocks, G == 32 ? 256 : G, 0, st>>>(a);
+                cudaError_t e = cudaGetLastError();
+                if (e != cudaSuccess || !a.partial) return e;
+                rms_gw_kernel<T><<<(a.dim + 31) / 32, 256, 0, st>>>(a.partial, blocks, a.dim, a.gw, a.w_f32);
+                return cudaGetLastError();
+            });
+        };
+        if (vec) return run(std::integral_constant<int, kN>{});
+        return run(std::integral_constant<int, 1>{});
+    });
+}
+
+}  // namespace mmltk

@@ -50,13 +50,14 @@ def extensions(debug_bounds: bool = False):
         CppExtension("mmltk_b200._native", host_src, include_dirs=inc + [os.path.join(ROOT, "csrc", "host")],
                      extra_compile_args={"cxx": CXX_FLAGS}, extra_link_args=["-lpthread", "-lz"]),
         CUDAExtension("mmltk_b200._kernels", kern_src, include_dirs=inc,
-                      extra_compile_args={"cxx": CXX_FLAGS, "nvcc": NVCC_FLAGS}),
+                      extra_compile_args={"cxx": CXX_FLAGS, "nvcc": NVCC_FLAGS}, extra_link_args=_stdcxx_args()),
     ]
     exts.append(_cudnn_extension(inc))
     if debug_bounds:
         exts.append(CUDAExtension("mmltk_b200._kernels_dbg", kern_src, include_dirs=inc,
                                   extra_compile_args={"cxx": CXX_FLAGS + DEBUG_FLAGS,
-                                                      "nvcc": NVCC_FLAGS + DEBUG_FLAGS}))
+                                                      "nvcc": NVCC_FLAGS + DEBUG_FLAGS},
+                                  extra_link_args=_stdcxx_args()))
     return exts
 
 
@@ -86,7 +87,13 @@ def _cudnn_extension(inc):
                          extra_compile_args={"cxx": CXX_FLAGS + ["-fvisibility=hidden", "-fvisibility-inlines-hidden"],
                                              "nvcc": NVCC_FLAGS},
                          extra_link_args=[f"-L{cudnn_lib}", "-l:libcudnn.so.9", f"-Wl,-rpath,{cudnn_lib}",
-                                          "-Wl,--no-as-needed", _shared_libstdcxx(), "-Wl,--as-needed"])
+                                          *_stdcxx_args()])
+
+
+def _stdcxx_args() -> list:
+    """Links the process's libstdc++ by path.  ``_kernels`` needs it too: an error message with a number in
+    it (an argument check that fails) goes through std::ostream, which crashed on the private copy."""
+    return ["-Wl,--no-as-needed", _shared_libstdcxx(), "-Wl,--as-needed"]
 
 
 def _shared_libstdcxx() -> str:

@@ -1,0 +1,135 @@
+"""The microscaled formats' plain definition (CPU) against a 64-bit one, their layout, and what the operators refuse."""
+import numpy as np
+import pytest
+import torch
+
+from mmltk_b200 import ops
+from mmltk_b200.ops import MXTensor
+
+from microscale_oracle import BLOCK, FORMATS, hard_rows, quantize, tensor_scale, unpack
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim", [1, 15, 32, 100, 257])
+def test_quantize_matches_64_bit_definition(fmt, dim):
+    x = hard_rows(dim)
+    g = None if fmt != "nvfp4" else torch.tensor([0.037])
+    t = ops.mx_quantize(x, fmt, g)
+    codes, byte, val = quantize(x.double().numpy(), fmt, None if g is None else g.item())
+    c, s = unpack(t)
+    np.testing.assert_array_equal(s, byte)
+    np.testing.assert_array_equal(np.where(np.isnan(val), 0, c), np.where(np.isnan(val), 0, codes))
+    # a value is code x scale (x g): products of few-bit factors, so one fp32 rounding at most (below its normals,
+    # half a step of 2^-149; 4 x 2^126, which a number just below 2^128 rounds to, is an infinity in fp32)
+    with np.errstate(over="ignore"):
+        want = val.astype(np.float32)
+    np.testing.assert_allclose(t.dequantize(torch.float32).numpy(), want, rtol=2.0 ** -23, atol=2.0 ** -149)
+
+
+def test_tensor_scale_is_found():
+    x = torch.randn(7, 65, generator=torch.Generator().manual_seed(1))
+    assert ops.mx_quantize(x, "nvfp4").global_scale.item() == tensor_scale(x.numpy())
+    for bad in (torch.zeros(2, 16), torch.full((2, 16), float("inf"))):
+        assert ops.mx_quantize(bad, "nvfp4").global_scale.item() == 1.0
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_layout_sizes(fmt):
+    t = ops.mx_quantize(torch.randn(2, 65, 130), fmt)
+    nb = -(-130 // BLOCK[fmt])
+    assert t.shape == (2, 65, 130) and t.rows == 130
+    assert t.codes.shape == (130, 144 if fmt == "mxfp8" else 80)
+    assert t.scales.shape == (2, -(-nb // 4), 32, 4, 4)
+    assert t.dequantize().shape == (2, 65, 130) and t.dequantize().dtype == torch.bfloat16
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("act", [None, "relu", "gelu"])
+def test_linear_definition(fmt, act):
+    gen = torch.Generator().manual_seed(2)
+    x, w, b = torch.randn(3, 5, 70, generator=gen), torch.randn(9, 70, generator=gen), torch.randn(9, generator=gen)
+    wq = ops.mx_quantize(w, fmt)
+    g = 1.0 if fmt == "nvfp4" else None
+    xv = quantize(x.view(-1, 70).double().numpy(), fmt, g)[2]
+    wv = wq.dequantize(torch.float32).double()
+    y = torch.from_numpy(xv) @ wv.t() + b.double()
+    y = {None: lambda v: v, "relu": torch.relu, "gelu": torch.nn.functional.gelu}[act](y).view(3, 5, 9)
+    got = ops.mx_linear(x, wq, b, act=act)
+    assert got.shape == (3, 5, 9) and got.dtype == torch.float32
+    # 70 products summed in fp32, none larger than the sum of magnitudes
+    bound = 72 * 2.0 ** -24 * (torch.from_numpy(np.abs(xv)) @ wv.abs().t() + b.abs()).max().item()
+    assert (got.double() - y).abs().max().item() <= 1.13 * bound      # |gelu'| <= 1.13
+    q = ops.mx_linear(x, wq, b, act=act, out_fmt="mxfp8")
+    assert isinstance(q, MXTensor) and q.shape == (3, 5, 9)
+    again = ops.mx_quantize(got, "mxfp8")
+    assert torch.equal(q.codes.view(torch.uint8), again.codes.view(torch.uint8)) and torch.equal(q.scales, again.scales)
+
+
+def _refusals(dev):
+    x = torch.randn(4, 64, device=dev)
+    w = ops.mx_quantize(torch.randn(8, 64, device=dev), "mxfp4")
+    wn = ops.mx_quantize(torch.randn(8, 64, device=dev), "nvfp4")
+    one = torch.ones(1, device=dev)
+    calls = [
+        lambda: ops.mx_quantize(x, "int4"),
+        lambda: ops.mx_quantize(x.double(), "mxfp4"),
+        lambda: ops.mx_quantize(x.long(), "mxfp4"),
+        lambda: ops.mx_quantize(x[0, 0], "mxfp4"),
+        lambda: ops.mx_quantize(x[:, :0], "mxfp4"),
+        lambda: ops.mx_quantize(x, "mxfp4", one),
+        lambda: ops.mx_quantize(x.clone().requires_grad_(), "mxfp8"),
+        lambda: ops.mx_linear(x[:, :32], w),
+        lambda: ops.mx_linear(x, w, act="tanh"),
+        lambda: ops.mx_linear(x, w, out_fmt="mxfp4"),
+        lambda: ops.mx_linear(x, w, out_fmt="mxfp8", out_dtype=torch.bfloat16),
+        lambda: ops.mx_linear(x, w, out_dtype=torch.float64),
+        lambda: ops.mx_linear(x, w, act_scale=one),
+        lambda: ops.mx_linear(wn, wn, act_scale=one),
+        lambda: ops.mx_linear(ops.mx_quantize(x, "mxfp8"), w),
+        lambda: ops.mx_linear(ops.mx_quantize(x[:, :32], "mxfp4"), w),
+        lambda: ops.rms_norm(x, torch.ones(32, device=dev)),
+        lambda: ops.rms_norm(x.double(), torch.ones(64, device=dev).double()),
+        lambda: ops.rms_norm(x[0, 0], torch.ones(1, device=dev)),
+        lambda: ops.add_rms_norm(x, x[:2], torch.ones(64, device=dev)),
+        lambda: ops.add_rms_norm(x, x.half(), torch.ones(64, device=dev)),
+        lambda: ops.rms_norm_quantized(x.clone().requires_grad_(), torch.ones(64, device=dev)),
+        lambda: ops.rms_norm_quantized(x, torch.ones(64, device=dev), fmt="fp4"),
+        lambda: ops.rms_norm_quantized(x, torch.ones(64, device=dev), global_scale=one),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            call()
+            pytest.fail(f"call {i} was accepted")
+
+
+def test_refusals_cpu():
+    _refusals("cpu")
+
+
+@pytest.mark.gpu
+def test_refusals_gpu(cuda_device):
+    _refusals(cuda_device)
+    x = torch.randn(4, 64, device=cuda_device)
+    w = ops.mx_quantize(torch.randn(8, 64, device=cuda_device), "mxfp4")
+    for call in (
+        lambda: ops.rms_norm(torch.zeros(2, 16385, device=cuda_device), torch.ones(16385, device=cuda_device)),
+        lambda: ops.rms_norm(x, torch.ones(64)),
+        lambda: ops.mx_linear(x.cpu(), w),
+        lambda: ops.mx_linear(x, w, torch.ones(8)),
+        lambda: ops.mx_linear(x, w, torch.ones(9, device=cuda_device)),
+        lambda: ops.mx_linear(x, MXTensor(w.codes[:4], w.scales, "mxfp4", (8, 64))),
+        lambda: ops.mx_linear(x, MXTensor(w.codes, w.scales[..., :2], "mxfp4", (8, 64))),
+        lambda: ops.mx_linear(x, MXTensor(w.codes.float(), w.scales, "mxfp4", (8, 64))),
+        lambda: MXTensor(w.codes, w.scales, "mxfp4", (9, 64)).dequantize(),
+        lambda: ops.mx_quantize(x, "nvfp4", torch.ones(1)),
+        lambda: ops.mx_quantize(x, "nvfp4", torch.ones(2, device=cuda_device)),
+    ):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            call()
+
+
+def test_an_error_message_with_a_number_reaches_python():
+    # formatted by the extension itself: needs the process's libstdc++ (it crashed on a private copy)
+    c = torch.zeros(2, 16, dtype=torch.uint8)
+    with pytest.raises(RuntimeError, match="unknown format 9"):
+        ops.kernels().mx_dequantize(c, c, None, 9, 2, 16, torch.float32)
