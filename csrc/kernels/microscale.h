@@ -46,7 +46,7 @@ struct RmsFwdArgs {
 cudaError_t launch_rms_fwd(Elt et, const RmsFwdArgs& a, cudaStream_t st);
 
 struct RmsBwdArgs {
-    const void* gy;       // optional (null: no gradient reaches y)
+    const void* gy;       // gradient of y
     const void* gh;       // optional gradient of h
     const void* h;        // what the norm read
     const void* w;

@@ -212,12 +212,10 @@ std::pair<torch::Tensor, torch::Tensor> norm_backward(const torch::Tensor& gy, c
     a.dim = static_cast<int>(hr.size(1));
     a.h = hr.data_ptr();
     a.ldh = row_pitch(hr);
-    torch::Tensor gyr, ghr;
-    if (gy.defined()) {
-        gyr = as_rows(gy);
-        a.gy = gyr.data_ptr();
-        a.ldgy = row_pitch(gyr);
-    }
+    const torch::Tensor gyr = as_rows(gy);
+    torch::Tensor ghr;
+    a.gy = gyr.data_ptr();
+    a.ldgy = row_pitch(gyr);
     if (gh.defined()) {
         ghr = as_rows(gh);
         a.gh = ghr.data_ptr();

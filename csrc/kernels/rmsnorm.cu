@@ -200,10 +200,26 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(Rm
 }
 
 // ---------------------------------------------------------------- backward
+// 16 bytes of a row as loaded: unpacked where they are used, so that a row's three inputs wait in 12
+// registers per vector
+template <typename T, int VEC>
+struct Raw {
+    uint4 w;
+    __device__ __forceinline__ void load(const T* p) { w = __ldcs(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void get(float* f) const { unpack16(w, f, T()); }
+};
+template <typename T>
+struct Raw<T, 1> {
+    T v;
+    __device__ __forceinline__ void load(const T* p) { v = *p; }
+    __device__ __forceinline__ void get(float* f) const { f[0] = to_f(v); }
+};
+
 // Persistent: a group of threads walks rows and keeps its columns' part of gw in registers; one partial
 // row per CTA, summed in a fixed order by rms_gw_kernel (no atomics: the same bits every run).
 template <typename T, int VEC, int kGroup, int KV>
-__global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_bwd_kernel(RmsBwdArgs a) {
+__global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 : (kGroup >= 512 ? 1024 / kGroup : 768 / kGroup))
+    rms_bwd_kernel(RmsBwdArgs a) {
     constexpr int kRows = kGroup == 32 ? 8 : 1;
     __shared__ float red[2][32];
     __shared__ float part[kGroup == 32 ? 8 * 32 * VEC : 1];
@@ -219,28 +235,29 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_bwd_kernel(Rm
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + sub; r < a.rows;
          r += static_cast<int64_t>(gridDim.x) * kRows, turn ^= 1) {
         const float rstd = a.rstd[r];
-        float hv[KV][VEC], gv[KV][VEC], ev[KV][VEC];
+        Raw<T, VEC> hv[KV], gv[KV], ev[KV];
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
             const int i = (k * kGroup + t) * VEC;
             if (i < a.dim) {
-                load_vec<T, VEC>(static_cast<const T*>(a.h) + r * a.ldh + i, hv[k]);
-                if (a.gy) load_vec<T, VEC>(static_cast<const T*>(a.gy) + r * a.ldgy + i, gv[k]);
-                if (a.gh) load_vec<T, VEC>(static_cast<const T*>(a.gh) + r * a.ldgh + i, ev[k]);
+                hv[k].load(static_cast<const T*>(a.h) + r * a.ldh + i);
+                gv[k].load(static_cast<const T*>(a.gy) + r * a.ldgy + i);
+                if (a.gh) ev[k].load(static_cast<const T*>(a.gh) + r * a.ldgh + i);
             }
         }
         float s = 0.f;
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
             const int i = (k * kGroup + t) * VEC;
-            if (i < a.dim && a.gy) {
-                float w[VEC];
+            if (i < a.dim) {
+                float w[VEC], h[VEC], g[VEC];
                 load_w<T, VEC>(a.w, a.w_f32, i, w);
+                hv[k].get(h);
+                gv[k].get(g);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    acc[k][e] = fmaf(gv[k][e], hv[k][e] * rstd, acc[k][e]);
-                    gv[k][e] *= w[e];
-                    s = fmaf(hv[k][e], gv[k][e], s);
+                    acc[k][e] = fmaf(g[e], h[e] * rstd, acc[k][e]);
+                    s = fmaf(h[e], g[e] * w[e], s);
                 }
             }
         }
@@ -250,13 +267,18 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_bwd_kernel(Rm
         for (int k = 0; k < KV; ++k) {
             const int i = (k * kGroup + t) * VEC;
             if (i < a.dim) {
-                float o[VEC];
+                float w[VEC], h[VEC], g[VEC];
+                load_w<T, VEC>(a.w, a.w_f32, i, w);
+                hv[k].get(h);
+                gv[k].get(g);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    o[e] = a.gy ? fmaf(rstd, gv[k][e], -c * hv[k][e]) : 0.f;
-                    if (a.gh) o[e] += ev[k][e];
+                for (int e = 0; e < VEC; ++e) g[e] = fmaf(rstd, g[e] * w[e], -c * h[e]);
+                if (a.gh) {
+                    ev[k].get(h);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) g[e] += h[e];
                 }
-                store_vec<T, VEC>(static_cast<T*>(a.gx) + r * a.dim + i, o);
+                store_vec<T, VEC>(static_cast<T*>(a.gx) + r * a.dim + i, g);
             }
         }
     }
@@ -333,6 +355,31 @@ cudaError_t by_width(int elems, Fn&& fn) {
     return cudaErrorInvalidValue;
 }
 
+// The backward keeps its part of gw besides three rows' vectors: at most two vectors a thread, which leaves
+// registers for 1024 threads an SM.
+template <int VEC, typename Fn>
+cudaError_t by_width_bwd(int elems, Fn&& fn) {
+    auto go = [&](auto g, auto kv) { return fn(g, kv); };
+#define MMLTK_RMS_WIDTH(G, KV) \
+    if (elems <= G * KV * VEC) return go(std::integral_constant<int, G>{}, std::integral_constant<int, KV>{})
+    if constexpr (VEC == 1) {
+        MMLTK_RMS_WIDTH(128, 8);
+        MMLTK_RMS_WIDTH(512, 8);
+        MMLTK_RMS_WIDTH(1024, 16);
+    } else {
+        MMLTK_RMS_WIDTH(32, 1);
+        MMLTK_RMS_WIDTH(32, 2);
+        MMLTK_RMS_WIDTH(128, 1);
+        MMLTK_RMS_WIDTH(128, 2);
+        MMLTK_RMS_WIDTH(256, 2);
+        MMLTK_RMS_WIDTH(512, 2);
+        MMLTK_RMS_WIDTH(1024, 2);
+        if constexpr (VEC == 4) MMLTK_RMS_WIDTH(1024, 4);
+    }
+#undef MMLTK_RMS_WIDTH
+    return cudaErrorInvalidValue;
+}
+
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace
@@ -368,31 +415,31 @@ cudaError_t launch_rms_fwd(Elt et, const RmsFwdArgs& a, cudaStream_t st) {
 }
 
 namespace {
-// CTAs of the backward: two or more an SM at these register counts, fewer for few rows
-int bwd_blocks(int64_t rows, int dim, int group) {
+// CTAs of the backward: 1024 threads an SM, fewer for few rows
+int bwd_blocks(int64_t rows, int group) {
     const int64_t per = group == 32 ? 8 : 1;
-    const int per_sm = group == 32 ? 4 : (group >= 512 ? 2 : 4);
+    const int per_sm = group == 32 ? 3 : (group >= 512 ? 1024 / group : 768 / group);
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, num_sms() * per_sm)));
 }
 }  // namespace
 
 int rms_bwd_partials(Elt, int64_t rows, int) {
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, num_sms() * 4)));
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, num_sms() * 8)));
 }
 
 cudaError_t launch_rms_bwd(Elt et, const RmsBwdArgs& a, cudaStream_t st) {
-    if (a.dim <= 0 || a.dim > kRmsMaxDim) return cudaErrorInvalidValue;
+    if (a.dim <= 0 || a.dim > kRmsMaxDim || !a.gy) return cudaErrorInvalidValue;
     return MMLTK_DISPATCH_ELT(et, [&]() -> cudaError_t {
         using T = elt_t;
         constexpr int kN = VecOf<T>::kN;
         const bool vec = a.dim % kN == 0 && aligned(a.h) && a.ldh % kN == 0 && aligned(a.w) &&
-                         (!a.gy || (a.ldgy % kN == 0 && aligned(a.gy))) &&
+                         a.ldgy % kN == 0 && aligned(a.gy) &&
                          (!a.gh || (a.ldgh % kN == 0 && aligned(a.gh)));
         auto run = [&](auto vc) -> cudaError_t {
             constexpr int VEC = decltype(vc)::value;
-            return by_width<VEC>(a.dim, [&](auto gc, auto kc) -> cudaError_t {
+            return by_width_bwd<VEC>(a.dim, [&](auto gc, auto kc) -> cudaError_t {
                 constexpr int G = decltype(gc)::value, KV = decltype(kc)::value;
-                const int blocks = bwd_blocks(a.rows, a.dim, G);
+                const int blocks = bwd_blocks(a.rows, G);
                 rms_bwd_kernel<T, VEC, G, KV><<<blocks, G == 32 ? 256 : G, 0, st>>>(a);
                 cudaError_t e = cudaGetLastError();
                 if (e != cudaSuccess || !a.partial) return e;
