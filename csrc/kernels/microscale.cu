@@ -41,6 +41,7 @@ __global__ void __launch_bounds__(kQThreads) mx_quantize_kernel(const T* __restr
     using Tr = Traits<F>;
     constexpr int kAtoms = kTileCols / (4 * Tr::kBlock);     // scale tiles of this CTA: 1 or 2
     __shared__ __align__(16) uint8_t tile[kAtoms * 512];
+    allow_next();
     // with amax the maximum was found by a pass in ascending order just before: going backwards, this pass
     // finds the end of x still in L2 (16384 x 8192 bf16)
     const int64_t unit = amax ? gridDim.x - 1 - blockIdx.x : blockIdx.x;

@@ -136,6 +136,11 @@ __device__ __forceinline__ float tensor_scale(uint32_t amax_bits) {
     return fmaxf(a / 2688.0f, 7.888609052210118e-31f);
 }
 
+// Overlap of a quantisation with the set-up of the product that reads it (programmatic dependent launch): the first
+// lets the next kernel start, the second, there, waits until everything launched before is complete.
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- 16-byte vectors of the three input types
 template <typename T>
 struct VecOf {

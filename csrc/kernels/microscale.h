@@ -82,7 +82,7 @@ struct MxGemmArgs {
 };
 cudaError_t launch_mx_gemm(const MxGemmArgs& a, cudaStream_t st);
 
-// Few tokens (m <= mx_few_max_tokens): one launch that also quantises x (x != null) in each CTA.
+// Few tokens (m <= kMxFewTokens, and x's slices fit shared memory): one launch that also quantises x (x != null).
 constexpr int kMxFewTokens = 64;
 struct MxFewArgs {
     MxGemmArgs g;
@@ -90,6 +90,7 @@ struct MxFewArgs {
     int64_t ldx;
     Elt x_elt;
 };
+bool mx_few_fits(MxFormat f, int m, int n, int k);
 cudaError_t launch_mx_few(const MxFewArgs& a, cudaStream_t st);
 
 }  // namespace mmltk

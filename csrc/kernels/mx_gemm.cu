@@ -11,23 +11,25 @@
 //   mxfp4  kind::mxf4,     2 scales: half a tile, chosen by the descriptor's scale id 0 / 2
 //   mxfp8  kind::mxf8f6f4, 1 scale:  a quarter, id 0 .. 3
 //
-// Persistent, ten warps: warp 0 loads (TMA: codes as 128-byte swizzled boxes, scale tiles as 512-byte
+// Persistent: warp 0 loads (TMA: codes as 128-byte swizzled boxes, scale tiles as 512-byte
 // rows), warp 1 copies each stage's scales to tensor memory (tcgen05.cp, ordered before the MMAs of the
-// same thread) and issues the MMAs, warps 2-9 are the epilogue.  Two accumulators let it run under the
-// next tile's products.  With 256 columns two accumulators and the scales do not fit the 512 columns of
-// tensor memory: the second starts at column 208, and the epilogue drains the 48 shared columns first.
+// same thread) and issues the MMAs, sixteen warps are the epilogue.  Two accumulators let it run under the
+// next tile's products, and two sets of scale columns let a stage's copies run under the MMAs before
+// them.  With 256 columns all of that does not fit the 512 columns of tensor memory: the accumulators
+// share some, and the epilogue drains the shared ones first.
 //
-// The quantised output (mxfp8) needs no second pass: a thread holds 32 consecutive columns of a row,
-// which are one scale block.
+// Large products run on CTA pairs (cta_group::2): 256 x 256 tiles, each CTA holding its 128 rows of x
+// and half of the tile's rows of w, and the scales of both (the tile's w scales are needed next to
+// each CTA's accumulator).  What bounds a product of this kind is the operands' way from L2: a
+// 128 x 256 tile of one CTA needs 54 KB per 512 tensor-core cycles, a pair's half 38 KB.
+//
+// The output leaves through tensor stores of 128-byte rows (whole lines; 32-byte sectors straight from
+// registers took as long as the rest of a short product together).  The quantised output (mxfp8) needs
+// no second pass: a thread has 32 consecutive columns of a row, one scale block.
 //
 // Every wait is bounded: on a time-out the kernel records which role gave up in a status word and
 // leaves, after releasing its tensor memory.
-#include <cudaTypedefs.h>
-
-#include <cstdio>
-
-#include "microscale.cuh"
-#include "tcgen05.cuh"
+#include "mx_mma.cuh"
 
 namespace mmltk {
 
@@ -36,88 +38,39 @@ namespace {
 using namespace mx;
 using namespace tc;
 
-constexpr int kThreads = 320;
-constexpr int kEpiWarps = 8;
-constexpr int kRowBytes = 128;                     // bytes of codes per row and stage
+constexpr int kEpiWarps = 16;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kATile = 128 * kRowBytes;
-constexpr int kStageTile = 32 * 64;                // staging of one 32-row chunk of the output
 constexpr int kMaxStages = 6;
 constexpr int kSmemMax = 227 * 1024;
 
-template <MxFormat F>
-struct Kind;
-template <>
-struct Kind<MxFormat::kMxFp4> {
-    static constexpr int kAtoms = 2, kElems = 256;     // scale tiles and elements of a stage
-    static constexpr uint32_t kDesc = (1u << 7) | (1u << 10) | (1u << 23);   // e2m1 x e2m1, e8m0 scales
-};
-template <>
-struct Kind<MxFormat::kNvFp4> {
-    static constexpr int kAtoms = 4, kElems = 256;
-    static constexpr uint32_t kDesc = (1u << 7) | (1u << 10);                // e2m1 x e2m1, e4m3 scales
-};
-template <>
-struct Kind<MxFormat::kMxFp8> {
-    static constexpr int kAtoms = 1, kElems = 128;
-    static constexpr uint32_t kDesc = 1u << 23;                              // e4m3 x e4m3, e8m0 scales
-};
-
-template <MxFormat F>
-__device__ __forceinline__ void mma_block(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
-                                          uint32_t sfb, uint32_t accumulate) {
-    if constexpr (F == MxFormat::kNvFp4) {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate));
-    } else if constexpr (F == MxFormat::kMxFp4) {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate));
-    } else {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate));
-    }
-}
-
-// One 32 x 16 byte scale tile from shared memory to 4 columns of tensor memory, in all four lane quarters.
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t smem) {
-    uint64_t d = static_cast<uint64_t>((smem >> 4) & 0x3fff);
-    d |= static_cast<uint64_t>(128 >> 4) << 32;       // 8-row groups 128 bytes apart; one 16-byte column
-    d |= 1ull << 46;
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
-}
-
-__device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint64_t* bar, void* dst, int c0, int c1, int c2) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
-            smem_u32(dst)),
-        "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
-        : "memory");
-}
-
-template <MxFormat F, int BN_>
+template <MxFormat F, int BN_, bool kPair, int kSize>     // kSize: bytes of an output element
 struct Cfg {
     static constexpr int BN = BN_;
     static constexpr int kAtoms = Kind<F>::kAtoms;
-    static constexpr int kBTile = BN * kRowBytes;
+    static constexpr int kRows = kPair ? 256 : 128;
+    static constexpr int kBRows = kPair ? BN / 2 : BN;          // rows of w that a CTA holds
+    static constexpr int kBTile = kBRows * kRowBytes;
     static constexpr int kSfA = kAtoms * 512;
     static constexpr int kSfB = (BN / 128) * kAtoms * 512;
     static constexpr int kStageBytes = kATile + kBTile + kSfA + kSfB;
-    static constexpr int kFixed = kEpiWarps * kStageTile + kEpiWarps * (BN / 2) * 4 + 1024 + 256;
+    // staging of a warp's 32 output rows: 128-byte rows are whole lines, but the pair's long products need the
+    // room for their stages
+    static constexpr int kBoxBytes = BN == 256 && kPair && kSize < 4 ? 64 : 128;
+    static constexpr int kBox = BN / 4 * kSize <= kBoxBytes ? BN / 4 : kBoxBytes / kSize;   // columns
+    static constexpr int kRow = kBox * kSize;
+    static constexpr int kStaging = 32 * kRow;
+    static constexpr int kFixed = kEpiWarps * kStaging + 4 * BN * 4 + 1024 + 256;
     static constexpr int kStages =
         (kSmemMax - kFixed) / kStageBytes < kMaxStages ? (kSmemMax - kFixed) / kStageBytes : kMaxStages;
     static constexpr size_t kSmemBytes = static_cast<size_t>(kStages) * kStageBytes + kFixed;
-    // tensor memory columns: accumulators at 0 and kAcc1, scales from kSfCol
-    static constexpr int kSfCols = kAtoms * 4 * (1 + BN / 128);
-    static constexpr int kTmemCols = BN == 256 ? 512 : 512;
-    static constexpr int kSfCol = 512 - 48;
-    static constexpr int kAcc1 = BN == 256 ? kSfCol - 256 : 128;
-    static constexpr bool kOverlap = BN == 256;
-    static_assert(kSfCols <= 48);
+    // tensor memory: accumulators at columns 0 and kAcc1, two sets of scales at the end
+    static constexpr int kSfSet = kAtoms * 4 * (1 + BN / 128);
+    static constexpr int kSfCol = 512 - 2 * kSfSet;
+    static constexpr int kAcc1 = kSfCol - BN < BN ? kSfCol - BN : BN;
+    static constexpr int kShared = (BN - kAcc1 + 31) / 32;      // 32-column chunks with columns of both accumulators
+    static constexpr int kSharers = (kShared * 32 + BN / 4 - 1) / (BN / 4);   // column quarters with such chunks
+    static_assert(kStages >= 2 && kBox % 32 == 0 && kAcc1 > 0 && kShared <= BN / 64);
 };
 
 struct __align__(8) Ctl {
@@ -132,76 +85,36 @@ struct __align__(8) Ctl {
 
 struct Sched {
     int m_tiles, n_tiles, ktiles, units;
-    // groups of 8 row tiles, column-major inside a group: the tiles in flight share operand rows in L2
-    __device__ void tile(int u, int& mt, int& nt) const {
-        const int per = 8 * n_tiles, g = u / per, rest = u % per;
-        const int height = min(8, m_tiles - 8 * g);
-        mt = 8 * g + rest % height;
-        nt = rest / height;
-    }
-};
-
-// Output of one warp's 32 x 32 chunk (lane = row).
-template <typename O>
-struct Out {
-    static constexpr int kCols = 64 / sizeof(O);       // columns of a 64-byte staging row: 32 or 16
-};
-
-template <typename O>
-__device__ __forceinline__ void store_chunk(const MxGemmArgs& g, unsigned char* buf, const CUtensorMap* map, bool tma,
-                                            int lane, const float* x, int col, int row0) {
-    constexpr int kCols = Out<O>::kCols;
-#pragma unroll
-    for (int part = 0; part < 32 / kCols; ++part) {
-        const int c0 = col + part * kCols;
-        if (c0 >= g.n) break;
-        if (tma && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        __syncwarp();
-        unsigned char* rowp = buf + lane * 64;
-        const int sw = (lane >> 1) & 3;     // 64-byte swizzle
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<uint4*>(rowp + ((c ^ sw) << 4)) = pack16(x + part * kCols + c * (16 / sizeof(O)), O());
-        if (tma) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-                asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map),
-                             "r"(smem_u32(buf)), "r"(c0), "r"(row0)
-                             : "memory");
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            }
+    uint32_t per, magic;          // tiles of a group of 8 row tiles, and 2^32 / per
+    // groups of 8 row tiles, column by column inside a group: the tiles in flight share operand rows in L2.
+    // (Every role walks the tiles; plain divisions here cost the loading warp a third of a short tile's time.)
+    __device__ void tile(uint32_t u, int& mt, int& nt) const {
+        uint32_t g = __umulhi(u, magic);
+        while (g * per > u) --g;
+        while ((g + 1) * per <= u) ++g;
+        const uint32_t rest = u - g * per, height = m_tiles - 8 * g;
+        if (height >= 8) {
+            mt = 8 * g + (rest & 7);
+            nt = rest >> 3;
         } else {
-            // rows that are no multiple of 16 bytes: 64-byte row segments, a lane per element
-            __syncwarp();
-            for (int r = 0; r < 32 && row0 + r < g.m; ++r)
-                for (int e = lane; e < kCols && c0 + e < g.n; e += 32) {
-                    const int byte = e * static_cast<int>(sizeof(O));
-                    const O* p = reinterpret_cast<const O*>(buf + r * 64 + (((byte >> 4) ^ ((r >> 1) & 3)) << 4) + (byte & 15));
-                    static_cast<O*>(g.y)[static_cast<int64_t>(row0 + r) * g.n + c0 + e] = *p;
-                }
-            __syncwarp();
+            mt = 8 * g + rest % height;
+            nt = rest / height;
         }
     }
-}
+};
 
-// mxfp8 output: the 32 columns are one scale block.  Returns the scale byte.
-__device__ __forceinline__ uint32_t store_chunk_q(const MxGemmArgs& g, unsigned char* buf, const CUtensorMap* map,
-                                                  int lane, float* x, int col, int row0) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        if (col + i >= g.n) x[i] = 0.f;
-        m = max(m, abs_bits(x[i]));
-    }
-    const BlockScale sc = pow2_scale<8>(__uint_as_float(m));
+// Staging tiles: 32 rows (lane = row) of kRow bytes in the tensor store's swizzle of that width.
+template <int kRow>
+__device__ __forceinline__ uint4* staged(unsigned char* buf, int row, int piece) {
+    const int sw = kRow == 128 ? row & 7 : (kRow == 64 ? (row >> 1) & 3 : (row >> 2) & 1);
+    return reinterpret_cast<uint4*>(buf + row * kRow) + (piece ^ sw);
+}
+// The staging tile may be written again: the last store from it has been read.
+__device__ __forceinline__ void staging_free(int lane) {
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
-    uint4* rowp = reinterpret_cast<uint4*>(buf + lane * 32);
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-        rowp[c] = make_uint4(cvt_e4m3x4(x + 16 * c, sc.inv), cvt_e4m3x4(x + 16 * c + 4, sc.inv),
-                             cvt_e4m3x4(x + 16 * c + 8, sc.inv), cvt_e4m3x4(x + 16 * c + 12, sc.inv));
+}
+__device__ __forceinline__ void staging_store(int lane, const CUtensorMap* map, const unsigned char* buf, int col, int row0) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0) {
@@ -210,152 +123,358 @@ __device__ __forceinline__ uint32_t store_chunk_q(const MxGemmArgs& g, unsigned 
                      : "memory");
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
+}
+
+// Output rows that are no multiple of 16 bytes: 32 x 32 values (a row's in w) through shared memory, 32 bytes of a
+// row at a time, so that a warp writes row segments.
+template <typename O>
+__device__ __forceinline__ void store_any(const MxGemmArgs& g, unsigned char* buf, int lane, const uint32_t* w, int col,
+                                          int row0) {
+    constexpr int kCols = 32 / sizeof(O);
+#pragma unroll
+    for (int part = 0; part < 32 / kCols; ++part) {
+        const int c = col + part * kCols + lane % kCols;
+        uint4* rowp = reinterpret_cast<uint4*>(buf + lane * 32);
+        rowp[0] = make_uint4(w[8 * part], w[8 * part + 1], w[8 * part + 2], w[8 * part + 3]);
+        rowp[1] = make_uint4(w[8 * part + 4], w[8 * part + 5], w[8 * part + 6], w[8 * part + 7]);
+        __syncwarp();
+        for (int r = lane / kCols; r < 32 && row0 + r < g.m; r += 32 / kCols)
+            if (c < g.n)
+                static_cast<O*>(g.y)[static_cast<int64_t>(row0 + r) * g.n + c] =
+                    reinterpret_cast<const O*>(buf + r * 32)[lane % kCols];
+        __syncwarp();
+    }
+}
+
+// ---------------------------------------------------------------- epilogue arithmetic, two columns an instruction
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pack2(float lo, float hi) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(f2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {    // keeps a NaN
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// GELU(x) = x Phi(x) = max(x, 0) - |x| Phi(-|x|), with Phi(-a) = exp(-a^2 / 2) Q(a).  Q(a) = erfcx(a / sqrt 2) / 2 is
+// smooth and slow: a polynomial of degree 10 on [0, 6], fitted to the least maximum of exp(-a^2 / 2) |error|
+// (Lawson's reweighted least squares on 4001 Chebyshev points; 6.6e-8, and 1.1e-7 with its fp32 roundings).
+// One exponential and six packed multiply-adds per value; an epilogue with the erf formula's exponential and
+// reciprocal per value took 15 us of the ViT's first MLP product (10400 x 1536).
+__device__ __forceinline__ f2 gelu2(f2 x) {
+    const f2 t = mul2(mul2(x, x), pack2(-0.72134752044448170f, -0.72134752044448170f));    // -x^2 / 2 in powers of two
+    const float2 xs = unpack2(x), ts = unpack2(t);
+    const f2 a = pack2(fminf(fabsf(xs.x), 6.f), fminf(fabsf(xs.y), 6.f));
+    constexpr float kQ[11] = {0.49999994f,    -0.39893651f,   0.249916792f,   -0.132513806f,    0.0611548945f,  -0.0243139397f,
+                              0.00793939643f, -0.00197462994f, 0.000339739083f, -3.52078676e-05f, 1.63169466e-06f};
+    f2 q = pack2(kQ[10], kQ[10]);
+#pragma unroll
+    for (int i = 9; i >= 0; --i) q = fma2(q, a, pack2(kQ[i], kQ[i]));
+    const f2 p = mul2(q, pack2(ex2(ts.x), ex2(ts.y)));
+    return fma2(mul2(a, pack2(-1.f, -1.f)), p, pack2(max_nan(xs.x, 0.f), max_nan(xs.y, 0.f)));
+}
+
+// Two values to the output's type, ReLU in the conversion where it has one.
+template <typename O, bool kRelu>
+__device__ __forceinline__ void convert2(f2 v, uint32_t* w) {
+    const float2 t = unpack2(v);
+    if constexpr (std::is_same_v<O, float>) {
+        w[0] = __float_as_uint(kRelu ? max_nan(t.x, 0.f) : t.x);
+        w[1] = __float_as_uint(kRelu ? max_nan(t.y, 0.f) : t.y);
+    } else if constexpr (std::is_same_v<O, __half>) {
+        if constexpr (kRelu) asm("cvt.rn.relu.f16x2.f32 %0, %1, %2;" : "=r"(*w) : "f"(t.y), "f"(t.x));
+        else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(*w) : "f"(t.y), "f"(t.x));
+    } else {
+        if constexpr (kRelu) asm("cvt.rn.relu.bf16x2.f32 %0, %1, %2;" : "=r"(*w) : "f"(t.y), "f"(t.x));
+        else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(*w) : "f"(t.y), "f"(t.x));
+    }
+}
+
+// mxfp8 output: the 32 columns at col are one scale block; codes to w, returns the scale byte.
+template <bool kRelu>
+__device__ __forceinline__ uint32_t quantize_chunk(const MxGemmArgs& g, f2* x, int col, uint32_t* w) {
+    if (col + 32 > g.n) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float2 t = unpack2(x[i]);
+            x[i] = pack2(col + 2 * i < g.n ? t.x : 0.f, col + 2 * i + 1 < g.n ? t.y : 0.f);
+        }
+    }
+    float m = 0.f;      // of the magnitudes, or of the positive values; keeps a NaN
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float2 t = unpack2(x[i]);
+        if constexpr (kRelu) asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(t.x), "f"(t.y));
+        else asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(t.x), "f"(t.y));
+    }
+    const BlockScale sc = pow2_scale<8>(fabsf(m));
+    const f2 inv = pack2(sc.inv, sc.inv);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float2 a = unpack2(mul2(x[2 * i], inv)), b = unpack2(mul2(x[2 * i + 1], inv));
+        unsigned short lo, hi;
+        if constexpr (kRelu) {
+            asm("cvt.rn.satfinite.relu.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(a.y), "f"(a.x));
+            asm("cvt.rn.satfinite.relu.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(b.y), "f"(b.x));
+        } else {
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(a.y), "f"(a.x));
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(b.y), "f"(b.x));
+        }
+        w[i] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+    }
     return sc.byte;
 }
 
-template <MxFormat F, int BN_, typename O, bool kQuantOut>
+// 32 accumulator columns of this thread's row on their way to registers; settled by tmem_settle
+__device__ __forceinline__ void tmem_issue32(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_settle(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+
+template <MxFormat F, int BN_, bool kPair, typename O, bool kQuantOut>
 __global__ void __launch_bounds__(kThreads, 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
-                   const __grid_constant__ CUtensorMap tmY, MxGemmArgs g, Sched sch, bool tma_store) {
-    using C = Cfg<F, BN_>;
+                   const __grid_constant__ CUtensorMap tmY, MxGemmArgs g, Sched sch, bool tensor_store) {
+    constexpr int kSize = kQuantOut ? 1 : static_cast<int>(sizeof(O));
+    using C = Cfg<F, BN_, kPair, kSize>;
     using K = Kind<F>;
     constexpr int BN = C::BN, kStages = C::kStages, kAtoms = C::kAtoms;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned char* tilesA = smem;
     unsigned char* tilesB = tilesA + kStages * kATile;
-    unsigned char* sfA = tilesB + kStages * C::kBTile;
+    unsigned char* staging = tilesB + kStages * C::kBTile;
+    unsigned char* sfA = staging + kEpiWarps * C::kStaging;
     unsigned char* sfB = sfA + kStages * C::kSfA;
-    unsigned char* staging = sfB + kStages * C::kSfB;
-    float* bias_s = reinterpret_cast<float*>(staging + kEpiWarps * kStageTile);
-    Ctl* ctl = reinterpret_cast<Ctl*>(bias_s + kEpiWarps * (BN / 2));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float* bias_s = reinterpret_cast<float*>(sfB + kStages * C::kSfB);
+    Ctl* ctl = reinterpret_cast<Ctl*>(bias_s + 4 * BN);
+    // values that the compiler can see are the same in a whole warp stay in uniform registers, which is where the
+    // asynchronous instructions take their operands from
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int rank = kPair ? blockIdx.x & 1 : 0;
+    const int first = kPair ? blockIdx.x >> 1 : blockIdx.x, step = kPair ? gridDim.x >> 1 : gridDim.x;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&ctl->full[s], 1);
             mbar_init(&ctl->empty[s], 1);
         }
+        // the epilogue warps of both CTAs of a pair arrive on the even CTA's barriers
         for (int b = 0; b < 2; ++b) {
             mbar_init(&ctl->acc_full[b], 1);
-            mbar_init(&ctl->acc_empty[b], kEpiWarps);
-            mbar_init(&ctl->shared_empty[b], kEpiWarps / 2);
+            mbar_init(&ctl->acc_empty[b], kEpiWarps * (kPair ? 2 : 1));
+            mbar_init(&ctl->shared_empty[b], 4 * C::kSharers * (kPair ? 2 : 1));
         }
         ctl->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)),
-                     "r"(C::kTmemCols));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (kPair) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)),
+                         "r"(512));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)),
+                         "r"(512));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (kPair) cluster_sync_all();   // the other CTA's barriers are initialised before anything targets them
     tc_fence_after();
-    const uint32_t tmem = ctl->tmem_base;
+    wait_previous();
+    constexpr uint32_t tmem = 0;                // all 512 columns are this CTA's: they start at 0
 
     if (warp == 0) {
-        if (lane == 0) {
-            int it = 0;
-            for (int u = blockIdx.x; u < sch.units; u += gridDim.x) {
-                int mt, nt;
-                sch.tile(u, mt, nt);
-                for (int kt = 0; kt < sch.ktiles; ++kt, ++it) {
-                    const int s = it % kStages;
-                    if (!mbar_wait(&ctl->empty[s], ((it / kStages) & 1) ^ 1, &ctl->abort)) {
+        const uint32_t elected = elect_lane();
+        const uint32_t sa = smem_u32(tilesA), sb = smem_u32(tilesB), pa = smem_u32(sfA), pb = smem_u32(sfB);
+        const uint32_t full0 = kPair ? mapa_shared(smem_u32(&ctl->full[0]), 0) : smem_u32(&ctl->full[0]);
+        int s = 0;
+        uint32_t phase = 1;
+        for (int u = first; u < sch.units; u += step) {
+            int mt, nt;
+            sch.tile(u, mt, nt);
+            const int rt = kPair ? 2 * mt + rank : mt;      // this CTA's tile of 128 rows
+            for (int kt = 0; kt < sch.ktiles; ++kt) {
+                if (!__all_sync(0xffffffffu, mbar_wait(&ctl->empty[s], phase, &ctl->abort))) {
+                    if (elected) {
                         ctl->abort = 1;
                         atomicCAS(g.status, 0, 1);
-                        goto producer_done;
                     }
-                    // boxes past an extent are zero-filled and count in full
-                    mbar_expect_tx(&ctl->full[s], C::kStageBytes);
-                    tma_load_2d(&tmA, &ctl->full[s], tilesA + s * kATile, kt * kRowBytes, mt * 128);
-                    tma_load_2d(&tmB, &ctl->full[s], tilesB + s * C::kBTile, kt * kRowBytes, nt * BN);
-                    tma_load_3d(&tmSA, &ctl->full[s], sfA + s * C::kSfA, 0, kt * kAtoms, mt);
-                    tma_load_3d(&tmSB, &ctl->full[s], sfB + s * C::kSfB, 0, kt * kAtoms, nt * (BN / 128));
+                    goto producer_done;
+                }
+                // boxes past an extent are zero-filled and count in full
+                if (rank == 0 && elected) mbar_expect_tx(&ctl->full[s], C::kStageBytes * (kPair ? 2 : 1));
+                const uint32_t bar = full0 + 8 * s;
+                load_2d<kPair>(elected, &tmA, bar, sa + s * kATile, kt * kRowBytes, rt * 128);
+                load_2d<kPair>(elected, &tmB, bar, sb + s * C::kBTile, kt * kRowBytes, nt * BN + rank * C::kBRows);
+                load_3d<kPair>(elected, &tmSA, bar, pa + s * C::kSfA, 0, kt * kAtoms, rt);
+                load_3d<kPair>(elected, &tmSB, bar, pb + s * C::kSfB, 0, kt * kAtoms, nt * (BN / 128));
+                if (++s == kStages) {
+                    s = 0;
+                    phase ^= 1;
                 }
             }
-        producer_done:;
         }
+    producer_done:;
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = K::kDesc | (static_cast<uint32_t>(BN >> 3) << 17) | (128u >> 4 << 24);
-            const uint32_t tsa = tmem + C::kSfCol, tsb = tsa + 4 * kAtoms;
-            int it = 0, local = 0;
-            for (int u = blockIdx.x; u < sch.units; u += gridDim.x, ++local) {
+        if (rank == 0) {
+            const uint32_t elected = elect_lane();
+            constexpr uint32_t idesc = K::kDesc | (static_cast<uint32_t>(BN >> 3) << 17) |
+                                       (static_cast<uint32_t>(C::kRows >> 4) << 24);
+            const uint32_t a0 = operand_lo(smem_u32(tilesA)), b0 = operand_lo(smem_u32(tilesB));
+            const uint32_t pa0 = smem_u32(sfA) >> 4, pb0 = smem_u32(sfB) >> 4;
+            const uint32_t empty0 = smem_u32(&ctl->empty[0]), accf0 = smem_u32(&ctl->acc_full[0]);
+            // the other CTA's barriers (shared::cluster addresses run on like the shared ones)
+            const uint32_t empty1 = kPair ? mapa_shared(empty0, 1) : 0, accf1 = kPair ? mapa_shared(accf0, 1) : 0;
+            int local = 0, s = 0;
+            uint32_t phase = 0, set = 0;
+            for (int u = first; u < sch.units; u += step, ++local) {
                 const int buf = local & 1;
-                bool ok = mbar_wait(&ctl->acc_empty[buf], ((local >> 1) & 1) ^ 1, &ctl->abort);
-                if (C::kOverlap && local > 0)
-                    ok = ok && mbar_wait(&ctl->shared_empty[buf ^ 1], ((local - 1) >> 1) & 1, &ctl->abort);
-                if (!ok) {
-                    ctl->abort = 1;
-                    atomicCAS(g.status, 0, 2);
-                    break;
-                }
+                bool ok = mbar_wait_cluster(&ctl->acc_empty[buf], ((local >> 1) & 1) ^ 1, &ctl->abort);
+                if (C::kShared && local > 0)
+                    ok = ok && mbar_wait_cluster(&ctl->shared_empty[buf ^ 1], ((local - 1) >> 1) & 1, &ctl->abort);
+                ok = __all_sync(0xffffffffu, ok);
                 tc_fence_after();
                 const uint32_t acc = tmem + buf * C::kAcc1;
-                for (int kt = 0; kt < sch.ktiles; ++kt, ++it) {
-                    const int s = it % kStages;
-                    if (!mbar_wait(&ctl->full[s], (it / kStages) & 1, &ctl->abort)) {
-                        ctl->abort = 1;
-                        atomicCAS(g.status, 0, 2);
-                        ok = false;
-                        break;
-                    }
+                int left = g.k;
+                uint32_t more = 0, ready = 0;
+                for (; ok && left > 0; left -= K::kElems) {
+                    if (!ready) ok = __all_sync(0xffffffffu, mbar_wait(&ctl->full[s], phase, &ctl->abort));
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t a = smem_u32(tilesA + s * kATile), b = smem_u32(tilesB + s * C::kBTile);
-                    const uint32_t pa = smem_u32(sfA + s * C::kSfA), pb = smem_u32(sfB + s * C::kSfB);
-                    // scale tile j: A at columns tsa + 4 j; B's row tiles side by side for each j
+                    // ask for the next stage now and look at the answer after this one's MMAs: a wait costs 170
+                    // cycles even on a full stage, and the tensor core's queue is too short to cover them
+                    const int s1 = s + 1 == kStages ? 0 : s + 1;
+                    const uint32_t phase1 = s + 1 == kStages ? phase ^ 1 : phase;
+                    const uint32_t seen = left > K::kElems ? mbar_test(&ctl->full[s1], phase1) : 0u;
+                    const uint32_t a = a0 + s * (kATile >> 4), b = b0 + s * (C::kBTile >> 4);
+                    const uint32_t pa = pa0 + s * (C::kSfA >> 4), pb = pb0 + s * (C::kSfB >> 4);
+                    // scale tile j: x's at columns tsa + 4 j; w's row tiles side by side for each j
+                    const uint32_t tsa = tmem + C::kSfCol + set, tsb = tsa + 4 * kAtoms;
 #pragma unroll
                     for (int j = 0; j < kAtoms; ++j) {
-                        copy_scales(tsa + 4 * j, pa + j * 512);
+                        copy_scales<kPair>(elected, tsa + 4 * j, pa + j * 32);
 #pragma unroll
                         for (int r = 0; r < BN / 128; ++r)
-                            copy_scales(tsb + (BN / 128) * 4 * j + 4 * r, pb + (r * kAtoms + j) * 512);
+                            copy_scales<kPair>(elected, tsb + (BN / 128) * 4 * j + 4 * r, pb + (r * kAtoms + j) * 32);
                     }
-                    // MMAs that only see padding are left out (their scales may be another row tile's)
-                    const int mmas = min(4, (g.k - kt * K::kElems + K::kElems / 4 - 1) / (K::kElems / 4));
+                    // MMAs that would only see padding are left out
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
-                        if (kk < mmas) {
+                        if (kk * (K::kElems / 4) < left) {
                             const int j = kk * kAtoms / 4;
                             const uint32_t id = F == MxFormat::kNvFp4 ? 0u : (F == MxFormat::kMxFp4 ? (kk & 1) * 2u : kk);
-                            mma_block<F>(acc, operand_desc<false>(a, kk), operand_desc<false>(b, kk),
-                                         idesc | (id << 4) | (id << 29), tsa + 4 * j, tsb + (BN / 128) * 4 * j,
-                                         (kt | kk) ? 1u : 0u);
+                            mma_block<F, kPair>(elected, acc, a + 2 * kk, b + 2 * kk, idesc | (id << 4) | (id << 29),
+                                                tsa + 4 * j, tsb + (BN / 128) * 4 * j, more);
+                            more = 1;
                         }
                     }
-                    tc_commit(&ctl->empty[s]);
+                    if constexpr (kPair) {
+                        commit<true>(elected, empty0 + 8 * s);
+                        commit<true>(elected, empty1 + 8 * s);
+                    } else {
+                        commit<false>(elected, empty0 + 8 * s);
+                    }
+                    set ^= C::kSfSet;
+                    s = s1;
+                    phase = phase1;
+                    ready = __all_sync(0xffffffffu, seen);
                 }
-                if (!ok) break;
-                tc_commit(&ctl->acc_full[buf]);
+                if (!ok) {
+                    if (elected) {
+                        ctl->abort = 1;
+                        atomicCAS(g.status, 0, 2);
+                    }
+                    break;
+                }
+                if constexpr (kPair) {
+                    commit<true>(elected, accf0 + 8 * buf);
+                    commit<true>(elected, accf1 + 8 * buf);
+                } else {
+                    commit<false>(elected, accf0 + 8 * buf);
+                }
             }
         }
     } else {
-        const int q = warp & 3, half = (warp - 2) >> 2;
-        constexpr int kHalf = BN / 2, kChunks = kHalf / 32;
-        unsigned char* buf_s = staging + (warp - 2) * kStageTile;
-        float* bias_w = bias_s + (warp - 2) * kHalf;
+        // sixteen warps (four a scheduler hide the latencies of a chunk): lane quarter q, column quarter part
+        const int q = warp & 3, part = (warp - 2) >> 2;
+        constexpr int kCols = BN / 4, kChunks = kCols / 32;
+        unsigned char* buf_s = staging + (warp - 2) * C::kStaging;
+        constexpr int kBox = C::kBox, kRow = C::kRow, kPieces = 32 * kSize / 16;
+        float* bias_w = bias_s + (warp - 2) * kCols;
         const float alpha = (g.x_g ? *g.x_g : 1.f) * (g.w_g ? *g.w_g : 1.f);
         const int ykt = kQuantOut ? static_cast<int>(mx_scale_tiles(MxFormat::kMxFp8, g.n)) : 0;
+        auto bias_at = [&](int col) {
+            if (!g.bias || col >= g.n) return 0.f;
+            return g.bias_elt == Elt::kF32 ? static_cast<const float*>(g.bias)[col]
+                   : g.bias_elt == Elt::kBF16 ? to_f(static_cast<const __nv_bfloat16*>(g.bias)[col])
+                                              : to_f(static_cast<const __half*>(g.bias)[col]);
+        };
+        int mt = 0, nt = 0, mt_next = 0, nt_next = 0;
+        float bias_r[kChunks];
+        if (first < sch.units) {
+            sch.tile(first, mt_next, nt_next);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) bias_r[c] = bias_at(nt_next * BN + part * kCols + 32 * c + lane);
+        }
         int local = 0;
-        for (int u = blockIdx.x; u < sch.units; u += gridDim.x, ++local) {
-            int mt, nt;
-            sch.tile(u, mt, nt);
-            const int row0 = mt * 128 + 32 * q, col0 = nt * BN + half * kHalf;
-            // this warp's columns of the bias, as fp32
+        for (int u = first; u < sch.units; u += step, ++local) {
+            mt = mt_next;
+            nt = nt_next;
+            const int row0 = (kPair ? 2 * mt + rank : mt) * 128 + 32 * q, col0 = nt * BN + part * kCols;
+            // this warp's columns of the bias; the next tile's are on their way meanwhile
             __syncwarp();
-            for (int i = lane; i < kHalf; i += 32) {
-                float b = 0.f;
-                if (g.bias && col0 + i < g.n)
-                    b = g.bias_elt == Elt::kF32 ? static_cast<const float*>(g.bias)[col0 + i]
-                        : g.bias_elt == Elt::kBF16 ? to_f(static_cast<const __nv_bfloat16*>(g.bias)[col0 + i])
-                                                   : to_f(static_cast<const __half*>(g.bias)[col0 + i]);
-                bias_w[i] = b;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) bias_w[32 * c + lane] = bias_r[c];
+            __syncwarp();
+            if (u + step < sch.units) {
+                sch.tile(u + step, mt_next, nt_next);
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) bias_r[c] = bias_at(nt_next * BN + part * kCols + 32 * c + lane);
             }
-            __syncwarp();
             const int buf = local & 1;
             if (!mbar_wait(&ctl->acc_full[buf], (local >> 1) & 1, &ctl->abort)) {
                 if (lane == 0) atomicCAS(g.status, 0, 3);
@@ -363,61 +482,77 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
             }
             tc_fence_after();
-            const uint32_t acc = tmem + buf * C::kAcc1 + (static_cast<uint32_t>(32 * q) << 16) + half * kHalf;
-            // the two chunks with columns that both accumulators use come first: the last two of the
-            // first accumulator's right half, the first two of the second's left half
-            const bool shares = C::kOverlap && half == (buf ^ 1);
-            const int first = (shares && buf == 0) ? kChunks - 2 : 0;
-            uint32_t bytes = 0;
-#pragma unroll 1
+            const uint32_t acc = tmem + buf * C::kAcc1 + (static_cast<uint32_t>(32 * q) << 16) + part * kCols;
+            // chunks with columns of both accumulators (the first one's last, the second one's first) come first
+            const int mine = buf ? min(kChunks, C::kShared - part * kChunks)
+                                 : min(kChunks, C::kShared - (3 - part) * kChunks);     // how many, if positive
+            uint32_t bytes = 0, freed = 0;
+#pragma unroll
             for (int i = 0; i < kChunks; ++i) {
-                const int c = (first + i) & (kChunks - 1);
+                const int c = buf ? i : kChunks - 1 - i;
                 const int col = col0 + 32 * c;
-                const bool live = col < g.n && row0 < g.m;
-                float v[32];
-                tmem_ld32(acc + 32 * c, v);
-                if (shares && i == 1) {
+                uint32_t v[32];
+                tmem_issue32(acc + 32 * c, v);
+                tmem_settle(v);
+                if ((C::kShared && mine == i + 1) || i == kChunks - 1) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&ctl->shared_empty[buf]);
-                }
-                if (i == kChunks - 1) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&ctl->acc_empty[buf]);
-                }
-                uint32_t byte = 0;
-                if (live) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float4 b = reinterpret_cast<const float4*>(bias_w + 32 * c)[j];
-                        v[4 * j] = fmaf(v[4 * j], alpha, b.x);
-                        v[4 * j + 1] = fmaf(v[4 * j + 1], alpha, b.y);
-                        v[4 * j + 2] = fmaf(v[4 * j + 2], alpha, b.z);
-                        v[4 * j + 3] = fmaf(v[4 * j + 3], alpha, b.w);
-                    }
-                    if (g.act == 1) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = gelu_fwd(v[j]);
-                    } else if (g.act == 2) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = fmaxf(v[j], 0.f);
-                    }
-                    if constexpr (kQuantOut) {
-                        byte = store_chunk_q(g, buf_s, &tmY, lane, v, col, row0);
-                        if (row0 + lane >= g.m) byte = 0;
-                    } else {
-                        store_chunk<O>(g, buf_s, &tmY, tma_store, lane, v, col, row0);
+                    if (lane == 0) {
+                        if (C::kShared && mine == i + 1) {
+                            if constexpr (kPair) mbar_arrive_remote(mapa_shared(smem_u32(&ctl->shared_empty[buf]), 0));
+                            else mbar_arrive(&ctl->shared_empty[buf]);
+                        }
+                        if (i == kChunks - 1) {
+                            if constexpr (kPair) mbar_arrive_remote(mapa_shared(smem_u32(&ctl->acc_empty[buf]), 0));
+                            else mbar_arrive(&ctl->acc_empty[buf]);
+                        }
                     }
                 }
-                if constexpr (kQuantOut) bytes |= byte << (8 * (c & 3));
+                if (col >= g.n || row0 >= g.m) continue;       // warp-uniform
+                f2 x[16];
+                const f2 alpha2 = pack2(alpha, alpha);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const ulonglong2 b = reinterpret_cast<const ulonglong2*>(bias_w + 32 * c)[j];
+                    x[2 * j] = fma2(pack2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])), alpha2, b.x);
+                    x[2 * j + 1] = fma2(pack2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])), alpha2, b.y);
+                }
+                if (g.act == 1) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) x[j] = gelu2(x[j]);
+                }
+                uint32_t w[8 * kSize];
+                if constexpr (kQuantOut) {
+                    const uint32_t byte = g.act == 2 ? quantize_chunk<true>(g, x, col, w) : quantize_chunk<false>(g, x, col, w);
+                    if (row0 + lane < g.m) bytes |= byte << (8 * c);
+                } else if (g.act == 2) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) convert2<O, true>(x[j], w + j * kSize / 2);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) convert2<O, false>(x[j], w + j * kSize / 2);
+                }
+                if (!tensor_store) {
+                    if constexpr (!kQuantOut) store_any<O>(g, buf_s, lane, w, col, row0);
+                    continue;
+                }
+                if (freed == 0 || kBox == 32) {
+                    staging_free(lane);
+                    freed = 1;
+                }
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j)
+                    *staged<kRow>(buf_s, lane, (kBox == 32 ? 0 : c * kPieces) + j) =
+                        make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                if (kBox == 32) staging_store(lane, &tmY, buf_s, col, row0);
             }
+            if (kBox > 32 && tensor_store && col0 < g.n && row0 < g.m) staging_store(lane, &tmY, buf_s, col0, row0);
             if constexpr (kQuantOut) {
-                // scale bytes of this row's blocks: four (two) neighbours, one store; zero past m and n
-                if (nt * BN / 128 + half * kHalf / 128 < ykt) {
+                // scale bytes of this row's blocks: one or two neighbours; zero past m and n
+                if (row0 / 128 < (g.m + 127) / 128 && col0 / 128 < ykt) {
                     uint8_t* p = static_cast<uint8_t*>(g.scales) + scale_offset(row0 + lane, col0 / 32, ykt);
-                    if constexpr (kChunks == 4) *reinterpret_cast<uint32_t*>(p) = bytes;
-                    else *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(bytes);
+                    if constexpr (kChunks == 2) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(bytes);
+                    else *p = static_cast<uint8_t>(bytes);
                 }
             }
         }
@@ -426,102 +561,95 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (kPair) cluster_sync_all();   // no CTA leaves while the pair's MMAs may still read its shared memory
     if (warp == 0) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols));
+        if constexpr (kPair)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    }();
-    return fn;
-}
-
-// Codes: bytes [rows, row_bytes] (pitch), boxes of 128 bytes x box_rows, 128-byte swizzle, zero fill.
-bool codes_map(CUtensorMap* map, const void* p, int64_t row_bytes, int64_t rows, int64_t pitch, int box_rows) {
-    auto fn = encode_fn();
-    if (!fn) return false;
-    cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(rows)};
-    cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
-    cuuint32_t box[2] = {kRowBytes, static_cast<cuuint32_t>(box_rows)}, es[2] = {1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, es,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-// Scales: [row tiles, tiles along k, 512 bytes], boxes of `atoms` tiles x `row_tiles`.
-bool scales_map(CUtensorMap* map, const void* p, int64_t rows, int kt, int atoms, int row_tiles) {
-    auto fn = encode_fn();
-    if (!fn) return false;
-    cuuint64_t dims[3] = {256, static_cast<cuuint64_t>(kt), static_cast<cuuint64_t>((rows + 127) / 128)};
-    cuuint64_t strides[2] = {512, static_cast<cuuint64_t>(kt) * 512};
-    cuuint32_t box[3] = {256, static_cast<cuuint32_t>(atoms), static_cast<cuuint32_t>(row_tiles)}, es[3] = {1, 1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(p), dims, strides, box, es,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-// Output: 32-row boxes of 64 bytes (64-byte swizzle) or, quantised, of 32 codes; stores past the extents are clipped.
-bool out_map(CUtensorMap* map, void* p, Elt e, bool quant, int64_t cols, int64_t rows, int64_t pitch) {
+// Output: boxes of 32 rows x box columns in the swizzle of their width; stores past the extents are clipped.
+bool out_map(CUtensorMap* map, void* p, Elt e, bool quant, int64_t cols, int64_t rows, int64_t pitch, int box_cols) {
     auto fn = encode_fn();
     if (!fn) return false;
     const CUtensorMapDataType dt = quant ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                    : e == Elt::kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : e == Elt::kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const int row = box_cols * (quant ? 1 : e == Elt::kF32 ? 4 : 2);
     cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
     cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
-    cuuint32_t box[2] = {(!quant && e == Elt::kF32) ? 16u : 32u, 32u}, es[2] = {1, 1};
+    cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), 32u}, es[2] = {1, 1};
     return fn(map, dt, 2, p, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              quant ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+              row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : (row == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B),
+              CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <MxFormat F, int BN, typename O, bool kQ>
+template <MxFormat F, int BN, bool kPair, typename O, bool kQ>
 cudaError_t launch(const MxGemmArgs& g, cudaStream_t st) {
-    using C = Cfg<F, BN>;
-    CUtensorMap ta, tb, sa, sb, ty{};
+    using C = Cfg<F, BN, kPair, kQ ? 1 : static_cast<int>(sizeof(O))>;
+    CUtensorMap ta, tb, sa, sb;
     const int64_t row_bytes = (static_cast<int64_t>(g.k) * mx_bits(F) + 7) / 8;
     const int kt = static_cast<int>(mx_scale_tiles(F, g.k));
-    const bool tma_store = kQ || (g.y_pitch % 16 == 0 && reinterpret_cast<uintptr_t>(g.y) % 16 == 0);
-    bool ok = codes_map(&ta, g.x_codes, row_bytes, g.m, g.x_pitch, 128) &&
-              codes_map(&tb, g.w_codes, row_bytes, g.n, g.w_pitch, BN) &&
-              scales_map(&sa, g.x_scales, g.m, kt, C::kAtoms, 1) &&
-              scales_map(&sb, g.w_scales, g.n, kt, C::kAtoms, BN / 128);
-    if (kQ) ok = ok && out_map(&ty, g.codes, g.out, true, g.y_pitch, g.m, g.y_pitch);
-    else if (tma_store) ok = ok && out_map(&ty, g.y, g.out, false, g.n, g.m, g.y_pitch);
-    if (!ok) return cudaErrorInvalidValue;
+    if (!codes_map(&ta, g.x_codes, row_bytes, g.m, g.x_pitch, 128) ||
+        !codes_map(&tb, g.w_codes, row_bytes, g.n, g.w_pitch, C::kBRows) ||
+        !scales_map(&sa, g.x_scales, g.m, kt, C::kAtoms, 1) ||
+        !scales_map(&sb, g.w_scales, g.n, kt, C::kAtoms, BN / 128))
+        return cudaErrorInvalidValue;
     Sched sch;
-    sch.m_tiles = (g.m + 127) / 128;
+    sch.m_tiles = (g.m + C::kRows - 1) / C::kRows;
     sch.n_tiles = (g.n + BN - 1) / BN;
     sch.ktiles = (g.k + Kind<F>::kElems - 1) / Kind<F>::kElems;
     sch.units = sch.m_tiles * sch.n_tiles;
-    auto kern = mx_gemm_kernel<F, BN, O, kQ>;
+    sch.per = 8u * sch.n_tiles;
+    sch.magic = static_cast<uint32_t>((uint64_t(1) << 32) / sch.per);
+    const bool tensor_store = kQ || (g.y_pitch % 16 == 0 && reinterpret_cast<uintptr_t>(g.y) % 16 == 0);
+    CUtensorMap ty{};
+    if (tensor_store && !out_map(&ty, kQ ? g.codes : g.y, g.out, kQ, kQ ? g.y_pitch : g.n, g.m, g.y_pitch, C::kBox))
+        return cudaErrorInvalidValue;
+    auto kern = mx_gemm_kernel<F, BN, kPair, O, kQ>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmemBytes));
     if (e != cudaSuccess) return e;
-    kern<<<std::min(sch.units, num_sms()), kThreads, C::kSmemBytes, st>>>(ta, tb, sa, sb, ty, g, sch, tma_store);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(kPair ? 2 * std::min(sch.units, num_sms() / 2) : std::min(sch.units, num_sms()));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = kPair ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, ta, tb, sa, sb, ty, g, sch, tensor_store);
 }
 
-template <MxFormat F, int BN>
+template <MxFormat F, int BN, bool kPair>
 cudaError_t by_output(const MxGemmArgs& g, cudaStream_t st) {
-    if (g.codes) return launch<F, BN, float, true>(g, st);
-    if (g.out == Elt::kBF16) return launch<F, BN, __nv_bfloat16, false>(g, st);
-    if (g.out == Elt::kF16) return launch<F, BN, __half, false>(g, st);
-    return launch<F, BN, float, false>(g, st);
+    if (g.codes) return launch<F, BN, kPair, float, true>(g, st);
+    if (g.out == Elt::kBF16) return launch<F, BN, kPair, __nv_bfloat16, false>(g, st);
+    if (g.out == Elt::kF16) return launch<F, BN, kPair, __half, false>(g, st);
+    return launch<F, BN, kPair, float, false>(g, st);
 }
 
 template <MxFormat F>
 cudaError_t by_tile(const MxGemmArgs& g, cudaStream_t st) {
-    // 256-column tiles move a third fewer operand bytes per product; 128 where they would leave SMs idle
-    const int64_t wide = static_cast<int64_t>((g.m + 127) / 128) * ((g.n + 255) / 256);
-    if (g.n > 128 && wide >= num_sms()) return by_output<F, 256>(g, st);
-    return by_output<F, 128>(g, st);
+    // Pairs where the reduction is long (8 stages) and the pairs get two tiles each: at 8192^3 they take 388 us where
+    // 128 x 256 tiles of single CTAs take 462 (mxfp8) and 222 against 314 (nvfp4); at K = 256 they lose (31200 x 2048:
+    // 46 us against 32), each tile's hand-overs crossing the pair.  Else the width whose waves cost less, a
+    // 256-column tile counting 1.75 of a 128-column one (31200 x 2048 x 256: 33.5 and 31; 10400 x 1536 x 384: 19.0
+    // and 19.8; 512 x 4096 x 4096: 10.7 and 14.1).
+    const int64_t sms = num_sms(), rt = (g.m + 127) / 128;
+    const int64_t pairs = (rt + 1) / 2 * ((g.n + 255) / 256);
+    if (g.k >= 8 * Kind<F>::kElems && pairs >= sms) return by_output<F, 256, true>(g, st);
+    const int64_t w128 = (rt * ((g.n + 127) / 128) + sms - 1) / sms, w256 = (rt * ((g.n + 255) / 256) + sms - 1) / sms;
+    if (7 * w256 < 4 * w128) return by_output<F, 256, false>(g, st);
+    return by_output<F, 128, false>(g, st);
 }
 
 }  // namespace

@@ -353,6 +353,21 @@ std::vector<torch::Tensor> mx_linear(OptTensor x, OptTensor x_codes, OptTensor x
     }
     if (rows && n) {
         a.status = mx_status_word(w_codes.device());
+        if (mx_few_fits(f, a.m, a.n, a.k)) {
+            MxFewArgs few{};
+            if (xr.defined()) {
+                few.x = xr.data_ptr();
+                few.ldx = row_pitch(xr);
+                few.x_elt = elt_of(xr, "mx_linear");
+            } else {
+                a.x_codes = xc.data_ptr();
+                a.x_scales = xs.data_ptr();
+            }
+            few.g = a;
+            check_cuda(launch_mx_few(few, cur_stream()), "mx_linear");
+            if (quant_out) return {codes, scales};
+            return {y};
+        }
         if (xr.defined()) {
             xc = new_codes(f, rows, k, w_codes);
             xs = new_scales(f, rows, k, w_codes);

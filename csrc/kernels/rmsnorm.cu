@@ -121,6 +121,7 @@ __device__ __forceinline__ void quantize_store(const float* v, int i, int64_t r,
 template <typename T, int VEC, int kGroup, int KV, bool kQuant>
 __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(RmsFwdArgs a) {
     __shared__ float red[32];
+    if (kQuant) allow_next();
     constexpr int kRows = kGroup == 32 ? 8 : 1;
     const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + (kGroup == 32 ? threadIdx.x >> 5 : 0);
     const int t = threadIdx.x & (kGroup - 1);
