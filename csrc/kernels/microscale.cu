@@ -3,11 +3,10 @@
 //   s = scale of a block from its largest magnitude, q = round(x / s) to the element type, value = q s (g)
 //
 // Memory-bound: 2 bytes in and 0.53 (4-bit) or 1.03 (8-bit) bytes out per 16-bit element.
-// One CTA takes 128 rows x 128 elements, the rows of one scale tile: a thread holds 16 consecutive
-// elements of each of the four rows r, r + 32, r + 64, r + 96, whose loads are all in flight together,
-// and whose scale bytes are neighbours in the tile.  The tile is put together in shared memory and
-// leaves in 16-byte stores; a tile built from byte stores of CTAs that run at different times would
-// reach DRAM in parts.
+// A thread takes 16 consecutive elements (one 32-byte load) of each of the four rows r, r + 32, r + 64,
+// r + 96: the four loads are in flight together, held as loaded, and the four rows' scale bytes are
+// neighbours in their tile.  The tiles' rows are put together in shared memory and leave as whole
+// sectors; a tile built from byte stores of CTAs that run at different times would reach DRAM in parts.
 #include "microscale.cuh"
 
 namespace mmltk {
@@ -16,88 +15,75 @@ namespace {
 
 using namespace mx;
 
-constexpr int kTileRows = 128, kTileCols = 128;
 constexpr int kQThreads = 256;
 
-// 16 elements at x + col (col a multiple of 16); elements at or past dim read as zero.
-template <typename T>
-__device__ __forceinline__ void load16(const T* x, int64_t col, int64_t dim, bool vec, float* v) {
-    if (vec && col + 16 <= dim) {
-        constexpr int kN = VecOf<T>::kN;
-#pragma unroll
-        for (int i = 0; i < 16 / kN; ++i) unpack16(reinterpret_cast<const uint4*>(x + col)[i], v + i * kN, T());
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = col + i < dim ? to_f(x[col + i]) : 0.f;
-    }
-}
-
-template <typename T, MxFormat F>
-__global__ void __launch_bounds__(kQThreads) mx_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t rows,
-                                                                int64_t dim, uint8_t* __restrict__ codes,
-                                                                int64_t pitch, uint8_t* __restrict__ scales, int kt,
-                                                                int64_t col_tiles, float* __restrict__ g_io,
-                                                                const uint32_t* __restrict__ amax, bool vec) {
+// kRow threads side by side in a row (8 or 32: 128 or 512 columns a CTA, of 4 x 32 or 4 x 8 rows).
+template <typename T, MxFormat F, int kRow>
+__global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 4 : 3)
+    mx_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t dim, uint8_t* __restrict__ codes,
+                       int64_t pitch, uint8_t* __restrict__ scales, int kt, int col_tiles, int units,
+                       float* __restrict__ g_io, const uint32_t* __restrict__ amax, int align) {
     using Tr = Traits<F>;
-    constexpr int kAtoms = kTileCols / (4 * Tr::kBlock);     // scale tiles of this CTA: 1 or 2
-    __shared__ __align__(16) uint8_t tile[kAtoms * 512];
+    constexpr int kCols = 16 * kRow, kLines = kQThreads / kRow;      // kLines: values of r % 32
+    constexpr int kAtoms = kCols / (4 * Tr::kBlock);                 // scale tiles across a CTA's columns
+    __shared__ __align__(16) uint8_t tile[kAtoms * kLines * 16];
     allow_next();
     // with amax the maximum was found by a pass in ascending order just before: going backwards, this pass
-    // finds the end of x still in L2 (16384 x 8192 bf16)
-    const int64_t unit = amax ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-    const int64_t rt = unit / col_tiles, ct = unit % col_tiles;
+    // finds the end of x still in L2
+    const int unit = amax ? units - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x);
+    const int ct = unit % col_tiles, line = unit / col_tiles;
     float g = 1.f;
     if constexpr (!Tr::kPow2) {
-        if (amax) {
-            g = tensor_scale(*amax);
-            if (unit == 0 && threadIdx.x == 0) *g_io = g;
-        } else if (g_io) {
-            g = *g_io;
-        }
+        if (!amax && g_io) g = *g_io;
     }
-    const int r32 = threadIdx.x >> 3, part = threadIdx.x & 7;
-    const int64_t col = ct * kTileCols + part * 16;
-    float v[4][16];
+    const int l = threadIdx.x / kRow, part = threadIdx.x % kRow;
+    const int64_t rt = static_cast<int64_t>(line) / (32 / kLines);
+    const int r32 = line % (32 / kLines) * kLines + l;
+    const int64_t r0 = rt * 128 + r32, col = static_cast<int64_t>(ct) * kCols + part * 16;
+    Raw16<T> raw[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        const int64_t r = rt * kTileRows + 32 * s + r32;
-        if (r < rows) {
-            load16(x + r * ld, col, dim, vec, v[s]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[s][i] = 0.f;
+        if (r0 + 32 * s < rows && col < dim) raw[s].load(x + (r0 + 32 * s) * ld, col, dim, align);
+        else raw[s].zero();
+    }
+    if constexpr (!Tr::kPow2) {
+        if (amax) {
+            wait_previous();      // for the maximum; x was complete before that pass began
+            g = tensor_scale(*amax);
+            if (unit == 0 && threadIdx.x == 0) *g_io = g;
         }
     }
     const int64_t pitch_cols = Tr::kBits == 4 ? 2 * pitch : pitch;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) m = max(m, abs_bits(v[s][i]));
+        uint32_t m = raw[s].amax_bits();
         if constexpr (Tr::kBlock == 32) m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
         const BlockScale sc = block_scale<F>(__uint_as_float(m), g);
-        const int64_t r = rt * kTileRows + 32 * s + r32;
+        const int64_t r = r0 + 32 * s;
+        float v[16];
+        raw[s].get(v);
         if (r < rows && col < pitch_cols) {
             if constexpr (Tr::kBits == 4) {
                 *reinterpret_cast<uint2*>(codes + r * pitch + col / 2) =
-                    make_uint2(cvt_e2m1x8(v[s], sc.inv), cvt_e2m1x8(v[s] + 8, sc.inv));
+                    make_uint2(cvt_e2m1x8(v, sc.inv), cvt_e2m1x8(v + 8, sc.inv));
             } else {
                 *reinterpret_cast<uint4*>(codes + r * pitch + col) =
-                    make_uint4(cvt_e4m3x4(v[s], sc.inv), cvt_e4m3x4(v[s] + 4, sc.inv), cvt_e4m3x4(v[s] + 8, sc.inv),
-                               cvt_e4m3x4(v[s] + 12, sc.inv));
+                    make_uint4(cvt_e4m3x4(v, sc.inv), cvt_e4m3x4(v + 4, sc.inv), cvt_e4m3x4(v + 8, sc.inv),
+                               cvt_e4m3x4(v + 12, sc.inv));
             }
         }
         if constexpr (Tr::kBlock == 32) {
-            if ((part & 1) == 0) tile[r32 * 16 + s * 4 + (part >> 1)] = static_cast<uint8_t>(sc.byte);
+            if ((part & 1) == 0) tile[((part >> 3) * kLines + l) * 16 + s * 4 + ((part >> 1) & 3)] = static_cast<uint8_t>(sc.byte);
         } else {
-            tile[(part >> 2) * 512 + r32 * 16 + s * 4 + (part & 3)] = static_cast<uint8_t>(sc.byte);
+            tile[((part >> 2) * kLines + l) * 16 + s * 4 + (part & 3)] = static_cast<uint8_t>(sc.byte);
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < kAtoms * 32; i += kQThreads) {
-        const int64_t atom = ct * kAtoms + i / 32;
+    for (int i = threadIdx.x; i < kAtoms * kLines; i += kQThreads) {
+        const int atom = ct * kAtoms + i / kLines;
         if (atom < kt)
-            reinterpret_cast<uint4*>(scales + (rt * kt + atom) * 512)[i % 32] = reinterpret_cast<const uint4*>(tile)[i];
+            reinterpret_cast<uint4*>(scales + (rt * kt + atom) * 512)[line % (32 / kLines) * kLines + i % kLines] =
+                reinterpret_cast<const uint4*>(tile)[i];
     }
 }
 
@@ -107,6 +93,7 @@ __global__ void __launch_bounds__(512) mx_amax_kernel(const T* __restrict__ x, i
                                                       uint32_t* __restrict__ amax, bool vec) {
     constexpr int kN = VecOf<T>::kN;
     uint32_t m = 0;
+    allow_next();
     if (vec) {   // whole 16-byte vectors: pitch, base and width all multiples
         const int64_t per_row = dim / kN, total = rows * per_row;
         const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
@@ -144,18 +131,21 @@ __global__ void __launch_bounds__(512) mx_amax_kernel(const T* __restrict__ x, i
     if ((threadIdx.x & 31) == 0 && m) atomicMax(amax, m);
 }
 
+// A thread writes 16 consecutive values (one 32-byte store of a 16-bit type); a CTA's y is a row of
+// CTAs, its x the columns.
 template <typename T, MxFormat F>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __restrict__ codes, int64_t pitch,
                                                             const uint8_t* __restrict__ scales, int kt,
                                                             const float* __restrict__ g_in, int64_t rows, int64_t dim,
-                                                            T* __restrict__ out, bool vec) {
+                                                            int parts, int part_bits, T* __restrict__ out, int align) {
     using Tr = Traits<F>;
-    const int64_t parts = (dim + 15) / 16;
     const float g = (!Tr::kPow2 && g_in) ? *g_in : 1.f;
-    const int64_t total = rows * parts;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t r = i / parts, col = (i % parts) * 16;
+    // 2^part_bits threads side by side in a row
+    const int part0 = threadIdx.x & ((1 << part_bits) - 1), line = threadIdx.x >> part_bits, lines = 256 >> part_bits;
+    for (int64_t r = static_cast<int64_t>(blockIdx.y) * lines + line; r < rows; r += static_cast<int64_t>(gridDim.y) * lines) {
+        const int part = (blockIdx.x << part_bits) + part0;
+        if (part >= parts) return;
+        const int64_t col = static_cast<int64_t>(part) * 16;
         const float s = scale_value<F>(scales[scale_offset(r, static_cast<int>(col / Tr::kBlock), kt)]);
         float v[16];
         if constexpr (Tr::kBits == 4) {
@@ -180,10 +170,13 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __res
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = v[e] * s * g;
         T* o = out + r * dim + col;
-        if (vec && col + 16 <= dim) {
-            constexpr int kN = VecOf<T>::kN;
+        constexpr int kN = VecOf<T>::kN;
+        if (align == 2 && col + 16 <= dim) {
 #pragma unroll
-            for (int e = 0; e < 16 / kN; ++e) reinterpret_cast<uint4*>(o)[e] = pack16(v + e * kN, T());
+            for (int e = 0; e < 16; e += 2 * kN) st_global_32(o + e, pack16(v + e, T()), pack16(v + e + kN, T()));
+        } else if (align && col + 16 <= dim) {
+#pragma unroll
+            for (int e = 0; e < 16; e += kN) *reinterpret_cast<uint4*>(o + e) = pack16(v + e, T());
         } else {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
@@ -204,29 +197,45 @@ cudaError_t by_format(MxFormat f, Fn&& fn) {
 cudaError_t launch_mx_quantize(Elt et, MxFormat f, const void* x, int64_t ld, int64_t rows, int64_t dim, void* codes,
                                void* scales, float* g, uint32_t* amax, cudaStream_t st) {
     if (rows <= 0 || dim <= 0) return cudaSuccess;
-    const int64_t row_tiles = (rows + kTileRows - 1) / kTileRows, col_tiles = (dim + kTileCols - 1) / kTileCols;
-    if (row_tiles * col_tiles >= (int64_t(1) << 31)) return cudaErrorInvalidValue;
+    // 512 columns a CTA where a row has them (rows' loads of 1 KB); 128 for narrow matrices, whose CTAs would idle
+    const int row_threads = dim > 256 ? 32 : 8;
+    const int64_t col_tiles = (dim + 16 * row_threads - 1) / (16 * row_threads);
+    const int64_t units = (rows + 127) / 128 * (row_threads / 8) * col_tiles;
+    if (units >= (int64_t(1) << 31)) return cudaErrorInvalidValue;
     return MMLTK_DISPATCH_ELT(et, [&]() -> cudaError_t {
         using T = elt_t;
         const int kN = 16 / static_cast<int>(sizeof(T));
-        const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld % kN == 0;
+        const int align = row_align(x, ld * static_cast<int64_t>(sizeof(T)));
         if (f == MxFormat::kNvFp4 && amax) {
             cudaError_t e = cudaMemsetAsync(amax, 0, sizeof(uint32_t), st);
             if (e != cudaSuccess) return e;
             const int64_t work = (rows * dim + 512 * kN * 4 - 1) / (512 * kN * 4);
             const int blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(work, num_sms() * 4)));
             mx_amax_kernel<T><<<blocks, 512, 0, st>>>(static_cast<const T*>(x), ld, rows, dim, amax,
-                                                      vec && dim % kN == 0);
+                                                      align && dim % kN == 0);
             e = cudaGetLastError();
             if (e != cudaSuccess) return e;
         }
         return by_format(f, [&](auto fc) -> cudaError_t {
             constexpr MxFormat F = decltype(fc)::value;
-            mx_quantize_kernel<T, F><<<static_cast<unsigned>(row_tiles * col_tiles), kQThreads, 0, st>>>(
-                static_cast<const T*>(x), ld, rows, dim, static_cast<uint8_t*>(codes), mx_pitch(f, dim),
-                static_cast<uint8_t*>(scales), static_cast<int>(mx_scale_tiles(f, dim)), col_tiles, g,
-                F == MxFormat::kNvFp4 ? amax : nullptr, vec);
-            return cudaGetLastError();
+            auto run = [&](auto kern) {
+                cudaLaunchConfig_t cfg{};
+                cfg.gridDim = dim3(static_cast<unsigned>(units));
+                cfg.blockDim = dim3(kQThreads);
+                cfg.stream = st;
+                cudaLaunchAttribute attr;
+                attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+                attr.val.programmaticStreamSerializationAllowed = 1;
+                cfg.attrs = &attr;
+                const uint32_t* found = F == MxFormat::kNvFp4 ? amax : nullptr;
+                cfg.numAttrs = found ? 1 : 0;      // only then does the kernel wait for the one before
+                return cudaLaunchKernelEx(&cfg, kern, static_cast<const T*>(x), ld, rows, dim, static_cast<uint8_t*>(codes),
+                                          mx_pitch(f, dim), static_cast<uint8_t*>(scales),
+                                          static_cast<int>(mx_scale_tiles(f, dim)), static_cast<int>(col_tiles),
+                                          static_cast<int>(units), g, found, align);
+            };
+            if (row_threads == 32) return run(mx_quantize_kernel<T, F, 32>);
+            return run(mx_quantize_kernel<T, F, 8>);
         });
     });
 }
@@ -234,16 +243,22 @@ cudaError_t launch_mx_quantize(Elt et, MxFormat f, const void* x, int64_t ld, in
 cudaError_t launch_mx_dequantize(Elt et, MxFormat f, const void* codes, const void* scales, const float* g,
                                  int64_t rows, int64_t dim, void* out, cudaStream_t st) {
     if (rows <= 0 || dim <= 0) return cudaSuccess;
-    const int64_t total = rows * ((dim + 15) / 16);
-    const int blocks = static_cast<int>(std::min<int64_t>((total + 255) / 256, static_cast<int64_t>(num_sms()) * 64));
+    const int64_t parts = (dim + 15) / 16;
+    if (parts >= (int64_t(1) << 30)) return cudaErrorInvalidValue;
+    int bits = 0;
+    while (bits < 8 && (int64_t(1) << bits) < parts) ++bits;
+    const int64_t lines = 256 >> bits;
+    const dim3 grid(static_cast<unsigned>((parts + (1 << bits) - 1) >> bits),
+                    static_cast<unsigned>(std::min<int64_t>((rows + lines - 1) / lines, 65535)));
     return MMLTK_DISPATCH_ELT(et, [&]() -> cudaError_t {
         using T = elt_t;
-        const bool vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && dim % (16 / static_cast<int>(sizeof(T))) == 0;
+        const int align = row_align(out, dim * static_cast<int64_t>(sizeof(T)));
         return by_format(f, [&](auto fc) -> cudaError_t {
             constexpr MxFormat F = decltype(fc)::value;
-            mx_dequantize_kernel<T, F><<<blocks, 256, 0, st>>>(
+            mx_dequantize_kernel<T, F><<<grid, 256, 0, st>>>(
                 static_cast<const uint8_t*>(codes), mx_pitch(f, dim), static_cast<const uint8_t*>(scales),
-                static_cast<int>(mx_scale_tiles(f, dim)), g, rows, dim, static_cast<T*>(out), vec);
+                static_cast<int>(mx_scale_tiles(f, dim)), g, rows, dim, static_cast<int>(parts), bits,
+                static_cast<T*>(out), align);
             return cudaGetLastError();
         });
     });

@@ -95,6 +95,11 @@ __device__ __forceinline__ BlockScale block_scale(float amax, float g) {
 
 // max that keeps a NaN (fmaxf drops it): on the bits of |x|, where NaN > infinity > every number
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 
 __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
@@ -102,12 +107,28 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
 __device__ __forceinline__ uint32_t cvt_e2m1x2(float lo, float hi) {
     return __nv_cvt_float2_to_fp4x2(make_float2(lo, hi), __NV_E2M1, cudaRoundNearest);
 }
+// products of neighbours with one factor, two an instruction
+__device__ __forceinline__ float2 scale2(const float* v, float inv) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(v[0]), "f"(v[1]), "f"(inv));
+    return r;
+}
 __device__ __forceinline__ uint32_t cvt_e4m3x4(const float* v, float inv) {
-    return cvt_e4m3x2(v[0] * inv, v[1] * inv) | (cvt_e4m3x2(v[2] * inv, v[3] * inv) << 16);
+    const float2 a = scale2(v, inv), b = scale2(v + 2, inv);
+    return cvt_e4m3x2(a.x, a.y) | (cvt_e4m3x2(b.x, b.y) << 16);
 }
 __device__ __forceinline__ uint32_t cvt_e2m1x8(const float* v, float inv) {
-    return cvt_e2m1x2(v[0] * inv, v[1] * inv) | (cvt_e2m1x2(v[2] * inv, v[3] * inv) << 8) |
-           (cvt_e2m1x2(v[4] * inv, v[5] * inv) << 16) | (cvt_e2m1x2(v[6] * inv, v[7] * inv) << 24);
+    const float2 a = scale2(v, inv), b = scale2(v + 2, inv), c = scale2(v + 4, inv), d = scale2(v + 6, inv);
+    uint32_t w;
+    asm("{\n\t.reg .b8 p, q, r, s;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 p, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 q, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 r, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 s, %8, %7;\n\t"
+        "mov.b32 %0, {p, q, r, s};\n\t}"
+        : "=r"(w)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y), "f"(d.x), "f"(d.y));
+    return w;
 }
 
 __device__ __forceinline__ float2 e4m3x2_to_f(uint32_t w) {
@@ -128,12 +149,13 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
     }
 }
 
-// Scale of a whole tensor (nvfp4) from its largest magnitude: puts the largest block scale at 448.
+// Scale of a whole tensor (nvfp4) from its largest magnitude, times 1 / (6 * 448) rounded to fp32: puts the largest
+// block scale at 448.
 // 2^-100 keeps 1 / (s g) finite; a tensor without a finite maximum keeps g = 1.
 __device__ __forceinline__ float tensor_scale(uint32_t amax_bits) {
     const float a = __uint_as_float(amax_bits);
     if (amax_bits == 0 || amax_bits >= 0x7f800000u) return 1.0f;
-    return fmaxf(a / 2688.0f, 7.888609052210118e-31f);
+    return fmaxf(a * (1.0f / 2688.0f), 7.888609052210118e-31f);
 }
 
 // Overlap of a quantisation with the set-up of the product that reads it (programmatic dependent launch): the first
@@ -184,6 +206,77 @@ __device__ __forceinline__ uint4 pack16(const float* f, __half) {
 __device__ __forceinline__ uint4 pack16(const float* f, float) {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
 }
+
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ void ld_global_32(const void* p, uint4* w) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0].x), "=r"(w[0].y), "=r"(w[0].z), "=r"(w[0].w), "=r"(w[1].x), "=r"(w[1].y), "=r"(w[1].z), "=r"(w[1].w)
+                 : "l"(p));
+}
+__device__ __forceinline__ void st_global_32(void* p, const uint4& a, const uint4& b) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z),
+                 "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
+}
+
+inline int row_align(const void* p, int64_t pitch_bytes) {
+    const uint64_t a = reinterpret_cast<uintptr_t>(p) | static_cast<uint64_t>(pitch_bytes);
+    return a % 32 == 0 ? 2 : (a % 16 == 0 ? 1 : 0);
+}
+
+// 16 consecutive elements of a row as they are stored; elements at or past dim are zeros.
+// align: the row starts at a multiple of 32 (2), of 16 (1) or of fewer bytes (0).
+template <typename T>
+struct Raw16 {
+    static constexpr int kVecs = static_cast<int>(sizeof(T));
+    uint4 w[kVecs];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) w[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(const T* x, int64_t col, int64_t dim, int align) {
+        if (align == 2 && col + 16 <= dim) {
+#pragma unroll
+            for (int i = 0; i < kVecs; i += 2) ld_global_32(reinterpret_cast<const uint4*>(x + col) + i, w + i);
+        } else if (align && col + 16 <= dim) {
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) w[i] = reinterpret_cast<const uint4*>(x + col)[i];
+        } else {
+            float f[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f[i] = col + i < dim ? to_f(x[col + i]) : 0.f;
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) w[i] = pack16(f + i * VecOf<T>::kN, T());     // exact: values of type T
+        }
+    }
+    __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) unpack16(w[i], v + i * VecOf<T>::kN, T());
+    }
+    // largest magnitude, as fp32 bits; keeps a NaN (as integers, 16-bit magnitudes order like their values)
+    __device__ __forceinline__ uint32_t amax_bits() const {
+        if constexpr (sizeof(T) == 2) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i)
+                m = max_u16x2(max_u16x2(max_u16x2(m, w[i].x & 0x7fff7fffu), w[i].y & 0x7fff7fffu),
+                              max_u16x2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu));
+            m = max(m & 0xffffu, m >> 16);
+            if constexpr (std::is_same_v<T, __half>) return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+            return m << 16;
+        } else {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i)
+                m = max(max(max(m, w[i].x & 0x7fffffffu), w[i].y & 0x7fffffffu), max(w[i].z & 0x7fffffffu, w[i].w & 0x7fffffffu));
+            return m;
+        }
+    }
+};
 
 }  // namespace mx
 }  // namespace mmltk

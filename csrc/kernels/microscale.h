@@ -82,15 +82,15 @@ struct MxGemmArgs {
 };
 cudaError_t launch_mx_gemm(const MxGemmArgs& a, cudaStream_t st);
 
-// Few tokens (m <= kMxFewTokens, and x's slices fit shared memory): one launch that also quantises x (x != null).
-constexpr int kMxFewTokens = 64;
+// Few tokens (where mx_few_fits says so): one launch that also quantises x (x != null).
+constexpr int kMxFewTokens = 32;
 struct MxFewArgs {
     MxGemmArgs g;
     const void* x;            // [m, k] (row pitch ldx elements) of type x_elt; null: g.x_codes / g.x_scales
     int64_t ldx;
     Elt x_elt;
 };
-bool mx_few_fits(MxFormat f, int m, int n, int k);
+bool mx_few_fits(MxFormat f, int m, int n, int k, bool quantised_x);
 cudaError_t launch_mx_few(const MxFewArgs& a, cudaStream_t st);
 
 }  // namespace mmltk

@@ -1,4 +1,4 @@
-// Product of few tokens (at most 64) with a microscaled weight, in one launch:
+// Product of few tokens (at most 32) with a microscaled weight, in one launch:
 //
 //   y[t, n] = act(g_x g_w sum_k x_q[t, k] w[n, k] + bias[n])
 //
@@ -40,28 +40,15 @@ struct __align__(8) FewCtl {
 
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
     float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
     return v;
 }
 
-// 16 elements of x at column col (a multiple of 16) of a row, zeros past k
-template <typename T>
-__device__ __forceinline__ void few_load16(const T* x, int col, int k, bool vec, float* v) {
-    if (vec && col + 16 <= k) {
-        constexpr int kN = VecOf<T>::kN;
-#pragma unroll
-        for (int i = 0; i < 16 / kN; ++i) unpack16(reinterpret_cast<const uint4*>(x + col)[i], v + i * kN, T());
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = col + i < k ? to_f(x[col + i]) : 0.f;
-    }
-}
-
-// kTok: tokens padded to the MMA's N (8, 16, 32 or 64).  T: x's element type, or uint8_t for quantised x.
+// kTok: tokens padded to the MMA's N (8, 16 or 32).  T: x's element type, or uint8_t for quantised x.
 template <MxFormat F, int kTok, typename T>
 __global__ void __launch_bounds__(kFewThreads, 2)
     mx_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmSW, MxFewArgs a,
-                  FewPlan pl, bool vec) {
+                  FewPlan pl, int align) {
     using K = Kind<F>;
     using Tr = Traits<F>;
     constexpr int kAtoms = K::kAtoms, kStage = kWTile + kAtoms * 512, kBTile = kTok * kRowBytes;
@@ -128,31 +115,54 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     } else {
         constexpr int kParts = K::kElems / 16;      // 16-element parts of a row and stage
         const float gx = (!Tr::kPow2 && g.x_g) ? *g.x_g : 1.f;
-        const int total = kts * g.m * kParts;       // (a multiple of 8: whole pairs of lanes)
-        for (int i0 = 0; i0 < total; i0 += kFewThreads) {
-            const int i = i0 + threadIdx.x;
-            const bool live = i < total;
-            const int part = i % kParts, t = live ? (i / kParts) % g.m : 0, st = live ? i / kParts / g.m : 0;
-            float v[16];
-            few_load16(static_cast<const T*>(a.x) + t * a.ldx, (kt0 + st) * K::kElems + part * 16, g.k, vec, v);
-            uint32_t m = 0;
+        // a thread keeps its part of the row and walks (stage, token); the loads of kAhead steps are in flight together
+        constexpr int kAhead = 2, kStep = kFewThreads / kParts;
+        const int part = threadIdx.x % kParts, total = kts * g.m;
+        int st = 0, t = threadIdx.x / kParts;
+        const int first = t;
+        while (t >= g.m && st < kts) {
+            t -= g.m;
+            ++st;
+        }
+        for (int i0 = 0; i0 < total; i0 += kAhead * kStep) {
+            Raw16<T> raw[kAhead];
+            int ts[kAhead], sts[kAhead];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) m = max(m, abs_bits(v[e]));
-            if constexpr (Tr::kBlock == 32) m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            const BlockScale sc = block_scale<F>(__uint_as_float(m), gx);
-            if (live) {
-                unsigned char* row = xs + st * kBTile + t * kRowBytes;
+            for (int u = 0; u < kAhead; ++u) {
+                ts[u] = t;
+                sts[u] = st;
+                if (i0 + u * kStep + first < total)
+                    raw[u].load(static_cast<const T*>(a.x) + t * a.ldx, (kt0 + st) * K::kElems + part * 16, g.k, align);
+                else
+                    raw[u].zero();
+                t += kStep;
+                while (t >= g.m && st < kts) {
+                    t -= g.m;
+                    ++st;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const bool live = i0 + u * kStep + first < total;
+                uint32_t m = raw[u].amax_bits();
+                if constexpr (Tr::kBlock == 32) m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                if (!live) continue;
+                float v[16];
+                raw[u].get(v);
+                const BlockScale sc = block_scale<F>(__uint_as_float(m), gx);
+                unsigned char* row = xs + sts[u] * kBTile + ts[u] * kRowBytes;
                 if constexpr (Tr::kBits == 4) {
-                    *reinterpret_cast<uint2*>(row + (((part >> 1) ^ (t & 7)) << 4) + (part & 1) * 8) =
+                    *reinterpret_cast<uint2*>(row + (((part >> 1) ^ (ts[u] & 7)) << 4) + (part & 1) * 8) =
                         make_uint2(cvt_e2m1x8(v, sc.inv), cvt_e2m1x8(v + 8, sc.inv));
                 } else {
-                    *reinterpret_cast<uint4*>(row + ((part ^ (t & 7)) << 4)) =
+                    *reinterpret_cast<uint4*>(row + ((part ^ (ts[u] & 7)) << 4)) =
                         make_uint4(cvt_e4m3x4(v, sc.inv), cvt_e4m3x4(v + 4, sc.inv), cvt_e4m3x4(v + 8, sc.inv),
                                    cvt_e4m3x4(v + 12, sc.inv));
                 }
                 const int b = part * 16 / Tr::kBlock;
                 if (Tr::kBlock == 16 || (part & 1) == 0)
-                    sfx[(st * kAtoms + (b >> 2)) * 512 + (t & 31) * 16 + (t >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(sc.byte);
+                    sfx[(sts[u] * kAtoms + (b >> 2)) * 512 + (ts[u] & 31) * 16 + (ts[u] >> 5) * 4 + (b & 3)] =
+                        static_cast<uint8_t>(sc.byte);
             }
         }
     }
@@ -236,34 +246,44 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 #pragma unroll
     for (int s = 0; s < kFewSplits; ++s) peers[s] = s < pl.splits ? mapa_shared(part_addr, s) : 0;
     const int ykt = g.codes ? static_cast<int>(mx_scale_tiles(MxFormat::kMxFp8, g.n)) : 0;
-    for (int i = rank * kFewThreads + threadIdx.x; i < g.m * 128; i += pl.splits * kFewThreads) {
-        const int t = i >> 7, n = nt * 128 + (i & 127);
-        float p[kFewSplits];
+    const int n = nt * 128 + (threadIdx.x & 127);
+    float bias = 0.f;
+    if (g.bias && n < g.n)
+        bias = g.bias_elt == Elt::kF32 ? static_cast<const float*>(g.bias)[n]
+               : g.bias_elt == Elt::kBF16 ? to_f(static_cast<const __nv_bfloat16*>(g.bias)[n])
+                                          : to_f(static_cast<const __half*>(g.bias)[n]);
+    const int step = pl.splits * (kFewThreads / 128);      // tokens between a thread's outputs
+    constexpr int kOuts = 2;                               // ... of which so many are read together
+    for (int t0 = (rank * kFewThreads + threadIdx.x) >> 7; t0 < g.m; t0 += kOuts * step) {
+        float p[kOuts][kFewSplits];
 #pragma unroll
-        for (int s = 0; s < kFewSplits; ++s) p[s] = s < pl.splits ? ld_cluster(peers[s] + i * 4) : 0.f;
-        float v = p[0];
+        for (int o = 0; o < kOuts; ++o)
 #pragma unroll
-        for (int s = 1; s < kFewSplits; ++s) v += p[s];
-        float b = 0.f;
-        if (g.bias && n < g.n)
-            b = g.bias_elt == Elt::kF32 ? static_cast<const float*>(g.bias)[n]
-                : g.bias_elt == Elt::kBF16 ? to_f(static_cast<const __nv_bfloat16*>(g.bias)[n])
-                                           : to_f(static_cast<const __half*>(g.bias)[n]);
-        v = fmaf(v, alpha, b);
-        if (g.act == 1) v = gelu_fwd(v);
-        else if (g.act == 2) v = v < 0.f ? 0.f : v;      // (keeps a NaN)
-        if (g.codes) {
-            if (n >= g.n) v = 0.f;
-            const BlockScale sc = pow2_scale<8>(__uint_as_float(__reduce_max_sync(0xffffffffu, abs_bits(v))));
-            if (n < g.y_pitch)
-                static_cast<uint8_t*>(g.codes)[t * g.y_pitch + n] = static_cast<uint8_t>(cvt_e4m3x2(v * sc.inv, 0.f));
-            if (lane == 0 && nt < ykt)
-                static_cast<uint8_t*>(g.scales)[scale_offset(t, n / 32, ykt)] = static_cast<uint8_t>(n < g.n ? sc.byte : 0u);
-        } else if (n < g.n) {
-            const int64_t o = static_cast<int64_t>(t) * g.n + n;
-            if (g.out == Elt::kBF16) static_cast<__nv_bfloat16*>(g.y)[o] = __float2bfloat16_rn(v);
-            else if (g.out == Elt::kF16) static_cast<__half*>(g.y)[o] = __float2half_rn(v);
-            else static_cast<float*>(g.y)[o] = v;
+            for (int s = 0; s < kFewSplits; ++s)
+                p[o][s] = (s < pl.splits && t0 + o * step < g.m) ? ld_cluster(peers[s] + ((t0 + o * step) * 128 + (threadIdx.x & 127)) * 4) : 0.f;
+#pragma unroll
+        for (int o = 0; o < kOuts; ++o) {
+            const int t = t0 + o * step;
+            if (t >= g.m) break;                           // (the same for a warp)
+            float v = p[o][0];
+#pragma unroll
+            for (int s = 1; s < kFewSplits; ++s) v += p[o][s];
+            v = fmaf(v, alpha, bias);
+            if (g.act == 1) v = gelu_fwd(v);
+            else if (g.act == 2) v = v < 0.f ? 0.f : v;    // (keeps a NaN)
+            if (g.codes) {
+                if (n >= g.n) v = 0.f;
+                const BlockScale sc = pow2_scale<8>(__uint_as_float(__reduce_max_sync(0xffffffffu, abs_bits(v))));
+                if (n < g.y_pitch)
+                    static_cast<uint8_t*>(g.codes)[t * g.y_pitch + n] = static_cast<uint8_t>(cvt_e4m3x2(v * sc.inv, 0.f));
+                if (lane == 0 && nt < ykt)
+                    static_cast<uint8_t*>(g.scales)[scale_offset(t, n / 32, ykt)] = static_cast<uint8_t>(n < g.n ? sc.byte : 0u);
+            } else if (n < g.n) {
+                const int64_t at = static_cast<int64_t>(t) * g.n + n;
+                if (g.out == Elt::kBF16) static_cast<__nv_bfloat16*>(g.y)[at] = __float2bfloat16_rn(v);
+                else if (g.out == Elt::kF16) static_cast<__half*>(g.y)[at] = __float2half_rn(v);
+                else static_cast<float*>(g.y)[at] = v;
+            }
         }
     }
     if (g.codes && rank == 0 && nt < ykt)     // rows that fill the scale tile
@@ -281,7 +301,7 @@ template <MxFormat F>
 FewPlan few_plan(int m, int n, int k) {
     constexpr int kAtoms = Kind<F>::kAtoms;
     FewPlan p{};
-    const int tok = m <= 8 ? 8 : (m <= 16 ? 16 : (m <= 32 ? 32 : 64));
+    const int tok = m <= 8 ? 8 : (m <= 16 ? 16 : 32);
     const int nts = (n + 127) / 128;
     p.ktiles = (k + Kind<F>::kElems - 1) / Kind<F>::kElems;
     // as many slices as give two CTAs an SM, at most 8 and at least one stage each
@@ -329,16 +349,14 @@ cudaError_t few_launch(const MxFewArgs& a, const FewPlan& pl, cudaStream_t st) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    const bool vec = sizeof(T) > 1 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.ldx * sizeof(T) % 16 == 0;
-    return cudaLaunchKernelEx(&cfg, kern, tw, sw, a, pl, vec);
+    return cudaLaunchKernelEx(&cfg, kern, tw, sw, a, pl, row_align(a.x, a.ldx * static_cast<int64_t>(sizeof(T))));
 }
 
 template <MxFormat F, typename T>
 cudaError_t few_by_tokens(const MxFewArgs& a, const FewPlan& pl, cudaStream_t st) {
     if (a.g.m <= 8) return few_launch<F, 8, T>(a, pl, st);
     if (a.g.m <= 16) return few_launch<F, 16, T>(a, pl, st);
-    if (a.g.m <= 32) return few_launch<F, 32, T>(a, pl, st);
-    return few_launch<F, 64, T>(a, pl, st);
+    return few_launch<F, 32, T>(a, pl, st);
 }
 
 template <MxFormat F>
@@ -353,8 +371,14 @@ cudaError_t few_by_input(const MxFewArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-bool mx_few_fits(MxFormat f, int m, int n, int k) {
+// Where it beats the tiles of mx_gemm.cu (graph replays, us, few / tiles): 16-bit x, 16 tokens, 8.8 / 10.4 (nvfp4
+// 4096 x 4096) and 19.0 / 22.7 (mxfp8 8192 x 8192); 32 tokens, 10.3 / 10.6 and 28.3 / 22.8: every CTA quantises its
+// slice of all tokens.  x quantised before, one token: 7.1 / 8.1 and 14.6 / 30.6, but 5.2 / 3.8 (mxfp4 1536 x 384) and
+// 5.9 / 5.5 (mxfp8 2048 x 1024), whose reduction is too short to cut.
+bool mx_few_fits(MxFormat f, int m, int n, int k, bool quantised_x) {
     if (m > kMxFewTokens) return false;
+    const int stages = (k + (f == MxFormat::kMxFp8 ? 127 : 255)) / (f == MxFormat::kMxFp8 ? 128 : 256);
+    if (quantised_x ? (m > 16 || stages < 16) : (m > 16 && stages > 16)) return false;
     if (f == MxFormat::kMxFp4) return few_plan<MxFormat::kMxFp4>(m, n, k).splits > 0;
     if (f == MxFormat::kNvFp4) return few_plan<MxFormat::kNvFp4>(m, n, k).splits > 0;
     return few_plan<MxFormat::kMxFp8>(m, n, k).splits > 0;

@@ -353,7 +353,7 @@ std::vector<torch::Tensor> mx_linear(OptTensor x, OptTensor x_codes, OptTensor x
     }
     if (rows && n) {
         a.status = mx_status_word(w_codes.device());
-        if (mx_few_fits(f, a.m, a.n, a.k)) {
+        if (mx_few_fits(f, a.m, a.n, a.k, !xr.defined())) {
             MxFewArgs few{};
             if (xr.defined()) {
                 few.x = xr.data_ptr();

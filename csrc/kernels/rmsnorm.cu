@@ -35,6 +35,27 @@ __device__ __forceinline__ void store_vec(T* p, const float* f) {
         *reinterpret_cast<uint4*>(p) = pack16(f, T());
     }
 }
+// A vector of a row as loaded: unpacked where it is used, so that a waiting row takes 4 registers per 16 bytes
+// (8 as fp32), which is what decides how many rows an SM has in flight.
+template <typename T, int VEC>
+struct Raw {
+    uint4 w;
+    __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = w; }
+    __device__ __forceinline__ void get(float* f) const { unpack16(w, f, T()); }
+    __device__ __forceinline__ void set(const float* f) { w = pack16(f, T()); }
+    __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
+};
+template <typename T>
+struct Raw<T, 1> {
+    T v;
+    __device__ __forceinline__ void load(const T* p) { v = *p; }
+    __device__ __forceinline__ void store(T* p) const { *p = v; }
+    __device__ __forceinline__ void get(float* f) const { f[0] = to_f(v); }
+    __device__ __forceinline__ void set(const float* f) { v = from_f<T>(f[0]); }
+    __device__ __forceinline__ void zero() { v = from_f<T>(0.f); }
+};
+
 // weights: x's type or fp32
 template <typename T, int VEC>
 __device__ __forceinline__ void load_w(const void* w, bool f32, int i, float* f) {
@@ -74,9 +95,11 @@ __device__ __forceinline__ void quantize_store(const float* v, int i, int64_t r,
                                                uint8_t* codes, uint8_t* scales, float g) {
     using Tr = Traits<F>;
     constexpr int kThreads = Tr::kBlock / VEC;      // threads of a block: 32 / 16, 8 / 4 or 4 / 2
-    uint32_t m = 0;
+    float top = fabsf(v[0]);      // keeps a NaN
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) m = max(m, abs_bits(v[e]));
+    for (int e = 1; e + 1 < VEC; e += 2) top = max3_abs_nan(top, v[e], v[e + 1]);
+    if constexpr (VEC % 2 == 0 && VEC > 1) top = max3_abs_nan(top, v[VEC - 1], v[VEC - 1]);
+    uint32_t m = abs_bits(top);
 #pragma unroll
     for (int o = 1; o < kThreads; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     const BlockScale sc = block_scale<F>(__uint_as_float(m), g);
@@ -134,41 +157,44 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(Rm
     }
     const T* xr = static_cast<const T*>(a.x) + r * a.ldx;
     const T* rr = a.res ? static_cast<const T*>(a.res) + r * a.ldr : nullptr;
-    float v[KV][VEC];
+    Raw<T, VEC> v[KV];
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
         const int i = (k * kGroup + t) * VEC;
-        if (i < a.dim) {
-            load_vec<T, VEC>(xr + i, v[k]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[k][e] = 0.f;
-        }
+        if (i < a.dim) v[k].load(xr + i);
+        else v[k].zero();
     }
+    float s = 0.f;
     if (rr) {
         T* hr = static_cast<T*>(a.h) + r * a.dim;
-        float u[KV][VEC];
+        Raw<T, VEC> u[KV];
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
             const int i = (k * kGroup + t) * VEC;
-            if (i < a.dim) load_vec<T, VEC>(rr + i, u[k]);
+            if (i < a.dim) u[k].load(rr + i);
         }
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
             const int i = (k * kGroup + t) * VEC;
             if (i < a.dim) {
                 // the norm sees the sum as it is stored, so that its backward can start from h
+                float f[VEC], e[VEC];
+                v[k].get(f);
+                u[k].get(e);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[k][e] = to_f(from_f<T>(v[k][e] + u[k][e]));
-                store_vec<T, VEC>(hr + i, v[k]);
+                for (int j = 0; j < VEC; ++j) f[j] += e[j];
+                v[k].set(f);
+                v[k].store(hr + i);
             }
         }
     }
-    float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < KV; ++k)
+    for (int k = 0; k < KV; ++k) {
+        float f[VEC];
+        v[k].get(f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) s = fmaf(v[k][e], v[k][e], s);
+        for (int j = 0; j < VEC; ++j) s = fmaf(f[j], f[j], s);
+    }
     s = group_sum<kGroup>(s, red);
     const float rstd = 1.f / sqrtf(s / static_cast<float>(a.dim) + a.eps);
     if (a.rstd && t == 0) a.rstd[r] = rstd;
@@ -178,12 +204,14 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(Rm
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
         const int i = (k * kGroup + t) * VEC;
+        float f[VEC];
+        v[k].get(f);
         if (i < a.dim) {
             float w[VEC];
             load_w<T, VEC>(a.w, a.w_f32, i, w);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[k][e] = v[k][e] * rstd * w[e];
-            if constexpr (!kQuant) store_vec<T, VEC>(static_cast<T*>(a.y) + r * a.dim + i, v[k]);
+            for (int j = 0; j < VEC; ++j) f[j] = f[j] * rstd * w[j];
+            if constexpr (!kQuant) store_vec<T, VEC>(static_cast<T*>(a.y) + r * a.dim + i, f);
         }
         if constexpr (kQuant) {
             if ((k * kGroup + (t & ~31)) * VEC >= span) continue;     // warp-uniform
@@ -191,31 +219,16 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(Rm
             uint8_t* scales = static_cast<uint8_t*>(a.scales);
             const int64_t pitch = mx_pitch(a.fmt, a.dim);
             if (a.fmt == MxFormat::kMxFp8)
-                quantize_store<MxFormat::kMxFp8, VEC>(v[k], i, r, pitch, kt, span, codes, scales, g);
+                quantize_store<MxFormat::kMxFp8, VEC>(f, i, r, pitch, kt, span, codes, scales, g);
             else if (a.fmt == MxFormat::kMxFp4)
-                quantize_store<MxFormat::kMxFp4, VEC>(v[k], i, r, pitch, kt, span, codes, scales, g);
+                quantize_store<MxFormat::kMxFp4, VEC>(f, i, r, pitch, kt, span, codes, scales, g);
             else
-                quantize_store<MxFormat::kNvFp4, VEC>(v[k], i, r, pitch, kt, span, codes, scales, g);
+                quantize_store<MxFormat::kNvFp4, VEC>(f, i, r, pitch, kt, span, codes, scales, g);
         }
     }
 }
 
 // ---------------------------------------------------------------- backward
-// 16 bytes of a row as loaded: unpacked where they are used, so that a row's three inputs wait in 12
-// registers per vector
-template <typename T, int VEC>
-struct Raw {
-    uint4 w;
-    __device__ __forceinline__ void load(const T* p) { w = __ldcs(reinterpret_cast<const uint4*>(p)); }
-    __device__ __forceinline__ void get(float* f) const { unpack16(w, f, T()); }
-};
-template <typename T>
-struct Raw<T, 1> {
-    T v;
-    __device__ __forceinline__ void load(const T* p) { v = *p; }
-    __device__ __forceinline__ void get(float* f) const { f[0] = to_f(v); }
-};
-
 // Persistent: a group of threads walks rows and keeps its columns' part of gw in registers; one partial
 // row per CTA, summed in a fixed order by rms_gw_kernel (no atomics: the same bits every run).
 template <typename T, int VEC, int kGroup, int KV>
@@ -429,7 +442,7 @@ int rms_bwd_partials(Elt, int64_t rows, int) {
 }
 
 cudaError_t launch_rms_bwd(Elt et, const RmsBwdArgs& a, cudaStream_t st) {
-    if (a.dim <= 0 || a.dim > kRmsMaxDim || !a.gy) return cudaErrorInvalidValue;
+    if (a.dim <= 0 || a.dim > kRmsMaxDim) return cudaErrorInvalidValue;
     return MMLTK_DISPATCH_ELT(et, [&]() -> cudaError_t {
         using T = elt_t;
         constexpr int kN = VecOf<T>::kN;

@@ -70,7 +70,7 @@ def quantize(x, fmt, g=None):
 
 def tensor_scale(x):
     a = np.abs(x).max()
-    return np.float32(1) if not np.isfinite(a) or a == 0 else max(np.float32(a) / np.float32(2688), np.float32(2.0 ** -100))
+    return np.float32(1) if not np.isfinite(a) or a == 0 else max(np.float32(a) * np.float32(1 / 2688), np.float32(2.0 ** -100))
 
 
 def unpack(t):
