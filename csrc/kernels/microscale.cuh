@@ -13,6 +13,8 @@
 #include <cuda_fp4.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "microscale.h"
 
@@ -221,6 +223,19 @@ __device__ __forceinline__ void st_global_32(void* p, const uint4& a, const uint
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z),
                  "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
                  : "memory");
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory; asked of each device once (a launch's host time counts).
+template <typename Kern>
+cudaError_t allow_smem(Kern kern, std::atomic<uint64_t>& done, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit);
+    return e;
 }
 
 inline int row_align(const void* p, int64_t pitch_bytes) {

@@ -53,7 +53,8 @@ struct RmsBwdArgs {
     const float* rstd;
     void* gx;
     void* gw;             // [dim] of w's type
-    float* partial;       // [rms_bwd_partials(...), dim] work space
+    float* partial;       // [rms_bwd_partials(...), dim] work space, null: no gw
+    int* status;          // set when a bounded wait gave up
     int64_t rows, ldgy, ldgh, ldh;
     int dim;
     bool w_f32;

@@ -334,7 +334,8 @@ cudaError_t few_launch(const MxFewArgs& a, const FewPlan& pl, cudaStream_t st) {
         !scales_map(&sw, g.w_scales, g.n, static_cast<int>(mx_scale_tiles(F, g.k)), Kind<F>::kAtoms, 1))
         return cudaErrorInvalidValue;
     auto kern = mx_few_kernel<F, kTok, T>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmemMax);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = allow_smem(kern, allowed, kFewSmemMax);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(pl.splits * ((g.n + 127) / 128));

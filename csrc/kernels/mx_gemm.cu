@@ -184,17 +184,30 @@ __device__ __forceinline__ float ex2(float x) {
 // (Lawson's reweighted least squares on 4001 Chebyshev points; 6.6e-8, and 1.1e-7 with its fp32 roundings).
 // One exponential and six packed multiply-adds per value; an epilogue with the erf formula's exponential and
 // reciprocal per value took 15 us of the ViT's first MLP product (10400 x 1536).
-__device__ __forceinline__ f2 gelu2(f2 x) {
-    const f2 t = mul2(mul2(x, x), pack2(-0.72134752044448170f, -0.72134752044448170f));    // -x^2 / 2 in powers of two
-    const float2 xs = unpack2(x), ts = unpack2(t);
-    const f2 a = pack2(fminf(fabsf(xs.x), 6.f), fminf(fabsf(xs.y), 6.f));
+template <int kPairs>
+__device__ __forceinline__ void gelu2(f2* x) {
     constexpr float kQ[11] = {0.49999994f,    -0.39893651f,   0.249916792f,   -0.132513806f,    0.0611548945f,  -0.0243139397f,
                               0.00793939643f, -0.00197462994f, 0.000339739083f, -3.52078676e-05f, 1.63169466e-06f};
-    f2 q = pack2(kQ[10], kQ[10]);
+    f2 a[kPairs], q[kPairs];
 #pragma unroll
-    for (int i = 9; i >= 0; --i) q = fma2(q, a, pack2(kQ[i], kQ[i]));
-    const f2 p = mul2(q, pack2(ex2(ts.x), ex2(ts.y)));
-    return fma2(mul2(a, pack2(-1.f, -1.f)), p, pack2(max_nan(xs.x, 0.f), max_nan(xs.y, 0.f)));
+    for (int j = 0; j < kPairs; ++j) {
+        const float2 xs = unpack2(x[j]);
+        a[j] = pack2(fmaxf(-fabsf(xs.x), -6.f), fmaxf(-fabsf(xs.y), -6.f));       // -min(|x|, 6)
+        q[j] = pack2(kQ[10], kQ[10]);
+    }
+#pragma unroll
+    for (int i = 9; i >= 0; --i) {
+        const float c = i & 1 ? -kQ[i] : kQ[i];                                   // Q as a polynomial of -|x|
+        const f2 c2 = pack2(c, c);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) q[j] = fma2(q[j], a[j], c2);
+    }
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+        const float2 xs = unpack2(x[j]), ts = unpack2(mul2(mul2(x[j], x[j]), pack2(-0.72134752044448170f, -0.72134752044448170f)));
+        const f2 p = mul2(q[j], pack2(ex2(ts.x), ex2(ts.y)));                     // exp(-x^2 / 2) in powers of two
+        x[j] = fma2(a[j], p, pack2(max_nan(xs.x, 0.f), max_nan(xs.y, 0.f)));
+    }
 }
 
 // Two values to the output's type, ReLU in the conversion where it has one.
@@ -370,17 +383,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             // the other CTA's barriers (shared::cluster addresses run on like the shared ones)
             const uint32_t empty1 = kPair ? mapa_shared(empty0, 1) : 0, accf1 = kPair ? mapa_shared(accf0, 1) : 0;
             int local = 0, s = 0;
-            uint32_t phase = 0, set = 0;
+            uint32_t phase = 0, set = 0, ready = 0;
             for (int u = first; u < sch.units; u += step, ++local) {
                 const int buf = local & 1;
-                bool ok = mbar_wait_cluster(&ctl->acc_empty[buf], ((local >> 1) & 1) ^ 1, &ctl->abort);
-                if (C::kShared && local > 0)
-                    ok = ok && mbar_wait_cluster(&ctl->shared_empty[buf ^ 1], ((local - 1) >> 1) & 1, &ctl->abort);
-                ok = __all_sync(0xffffffffu, ok);
+                // the accumulator was read two tiles ago, the columns it shares in the last one (both asked for together)
+                const uint32_t phase_a = ((local >> 1) & 1) ^ 1, phase_s = ((local - 1) >> 1) & 1;
+                const bool shared = C::kShared && local > 0;
+                const uint32_t free_s = shared ? mbar_try_wait_cluster(&ctl->shared_empty[buf ^ 1], phase_s) : 1u;
+                const uint32_t free_a = mbar_try_wait_cluster(&ctl->acc_empty[buf], phase_a);
+                bool ok = true;
+                if (!__all_sync(0xffffffffu, free_a & free_s)) {
+                    ok = mbar_wait_cluster(&ctl->acc_empty[buf], phase_a, &ctl->abort);
+                    if (shared) ok = ok && mbar_wait_cluster(&ctl->shared_empty[buf ^ 1], phase_s, &ctl->abort);
+                    ok = __all_sync(0xffffffffu, ok);
+                }
                 tc_fence_after();
                 const uint32_t acc = tmem + buf * C::kAcc1;
                 int left = g.k;
-                uint32_t more = 0, ready = 0;
+                uint32_t more = 0;
                 for (; ok && left > 0; left -= K::kElems) {
                     if (!ready) ok = __all_sync(0xffffffffu, mbar_wait(&ctl->full[s], phase, &ctl->abort));
                     if (!ok) break;
@@ -389,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // cycles even on a full stage, and the tensor core's queue is too short to cover them
                     const int s1 = s + 1 == kStages ? 0 : s + 1;
                     const uint32_t phase1 = s + 1 == kStages ? phase ^ 1 : phase;
-                    const uint32_t seen = left > K::kElems ? mbar_test(&ctl->full[s1], phase1) : 0u;
+                    const uint32_t seen = mbar_test(&ctl->full[s1], phase1);
                     const uint32_t a = a0 + s * (kATile >> 4), b = b0 + s * (C::kBTile >> 4);
                     const uint32_t pa = pa0 + s * (C::kSfA >> 4), pb = pb0 + s * (C::kSfB >> 4);
                     // scale tile j: x's at columns tsa + 4 j; w's row tiles side by side for each j
@@ -519,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (g.act == 1) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) x[j] = gelu2(x[j]);
+                    for (int j = 0; j < 16; j += 4) gelu2<4>(x + j);
                 }
                 uint32_t w[8 * kSize];
                 if constexpr (kQuantOut) {
@@ -611,7 +631,8 @@ cudaError_t launch(const MxGemmArgs& g, cudaStream_t st) {
     if (tensor_store && !out_map(&ty, kQ ? g.codes : g.y, g.out, kQ, kQ ? g.y_pitch : g.n, g.m, g.y_pitch, C::kBox))
         return cudaErrorInvalidValue;
     auto kern = mx_gemm_kernel<F, BN, kPair, O, kQ>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmemBytes));
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = allow_smem(kern, allowed, static_cast<int>(C::kSmemBytes));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(kPair ? 2 * std::min(sch.units, num_sms() / 2) : std::min(sch.units, num_sms()));

@@ -89,7 +89,8 @@ int* mx_status_word(const torch::Device& dev) {
     return t.data_ptr<int>();
 }
 
-// Non-zero when a product on this device gave up a bounded wait (1 loads, 2 MMA, 3 epilogue); clears it.
+// Non-zero when a kernel on this device gave up a bounded wait (products: 1 loads, 2 MMA, 3 epilogue; 4 norm
+// backward); clears it.
 int64_t mx_status(int64_t device) {
     const torch::Device dev(torch::kCUDA, static_cast<c10::DeviceIndex>(device));
     at::cuda::CUDAGuard guard(dev);
@@ -224,6 +225,7 @@ std::pair<torch::Tensor, torch::Tensor> norm_backward(const torch::Tensor& gy, c
     a.w = w.data_ptr();
     a.w_f32 = w.scalar_type() == torch::kFloat32 && h.scalar_type() != torch::kFloat32;
     a.rstd = rstd.data_ptr<float>();
+    a.status = mx_status_word(h.device());
     auto gx = torch::empty(h.sizes(), h.options());
     a.gx = gx.data_ptr();
     torch::Tensor gw, partial;

@@ -12,12 +12,15 @@
 // the pitch or an address is not a multiple of 16 bytes), so the 4 or 8 threads of a scale block
 // are neighbours in a warp and find its maximum with two or three shuffles.
 #include "microscale.cuh"
+#include "tcgen05.cuh"
 
 namespace mmltk {
 
 namespace {
 
 using namespace mx;
+
+constexpr int kRingStages = 8;
 
 template <typename T, int VEC>
 __device__ __forceinline__ void load_vec(const T* p, float* f) {
@@ -322,6 +325,113 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 
     }
 }
 
+// The same for rows of more than a warp: the inputs come through a ring of rows in shared memory (bulk asynchronous
+// copies), so what is in flight does not depend on registers; a row's stage is loaded again after the next row's
+// sum, when every thread has left it.  bf16, us (TB/s; loads into registers): 16384 x 8192 171 (6.3; 197), 32768 x 4096
+// 166 (6.5; 198), 65536 x 1024 101 (5.3; 119): a row of 1024 leaves little work between its two barriers.
+template <typename T, int kThreads, int KV>
+__global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, int stages) {
+    constexpr int VEC = VecOf<T>::kN;
+    extern __shared__ __align__(128) unsigned char ring[];
+    __shared__ float red[2][32];
+    __shared__ uint64_t full[kRingStages];
+    __shared__ int abort;
+    const int t = threadIdx.x;
+    const uint32_t row_bytes = static_cast<uint32_t>(a.dim) * sizeof(T);
+    const int inputs = a.gh ? 3 : 2;
+    const int64_t first = blockIdx.x, step = gridDim.x;
+    const int count = first < a.rows ? static_cast<int>((a.rows - 1 - first) / step) + 1 : 0;
+    if (t == 0) {
+        for (int s = 0; s < stages; ++s) tc::mbar_init(&full[s], 1);
+        abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    auto load = [&](int j) {     // (thread 0) row j of this CTA
+        const int s = j % stages;
+        const int64_t r = first + j * step;
+        const uint32_t dst = tc::smem_u32(ring) + s * 3 * row_bytes, bar = tc::smem_u32(&full[s]);
+        tc::mbar_expect_tx(&full[s], inputs * row_bytes);
+        const T* src[3] = {static_cast<const T*>(a.h) + r * a.ldh, static_cast<const T*>(a.gy) + r * a.ldgy,
+                           static_cast<const T*>(a.gh) + r * a.ldgh};
+        for (int i = 0; i < inputs; ++i)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                             dst + i * row_bytes),
+                         "l"(src[i]), "r"(row_bytes), "r"(bar)
+                         : "memory");
+    };
+    if (t == 0)
+        for (int j = 0; j < min(count, stages - 1); ++j) load(j);
+    float acc[KV][VEC], w[KV][VEC];
+#pragma unroll
+    for (int k = 0; k < KV; ++k) {
+        const int i = (k * kThreads + t) * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[k][e] = w[k][e] = 0.f;
+        if (i < a.dim) load_w<T, VEC>(a.w, a.w_f32, i, w[k]);
+    }
+    const float inv_dim = 1.f / static_cast<float>(a.dim);
+    for (int j = 0; j < count; ++j) {
+        const int s = j % stages;
+        const int64_t r = first + j * step;
+        const float rstd = a.rstd[r];
+        const bool here = tc::mbar_wait(&full[s], (j / stages) & 1, &abort);
+        const T* row = reinterpret_cast<const T*>(ring + s * 3 * row_bytes);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < KV; ++k) {
+            const int i = (k * kThreads + t) * VEC;
+            if (i < a.dim) {
+                float h[VEC], g[VEC];
+                load_vec<T, VEC>(row + i, h);
+                load_vec<T, VEC>(row + a.dim + i, g);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    acc[k][e] = fmaf(g[e], h[e] * rstd, acc[k][e]);
+                    sum = fmaf(h[e], g[e] * w[k][e], sum);
+                }
+            }
+        }
+        if (!here) {
+            abort = 1;
+            atomicCAS(a.status, 0, 4);
+        }
+        sum = group_sum<kThreads>(sum, red[j & 1]);
+        if (abort) break;                        // (seen by all after the barrier in group_sum)
+        if (t == 0 && j + stages - 1 < count) load(j + stages - 1);
+        const float c = sum * inv_dim * rstd * rstd * rstd;
+#pragma unroll
+        for (int k = 0; k < KV; ++k) {
+            const int i = (k * kThreads + t) * VEC;
+            if (i < a.dim) {
+                float h[VEC], g[VEC];
+                load_vec<T, VEC>(row + i, h);
+                load_vec<T, VEC>(row + a.dim + i, g);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) g[e] = fmaf(rstd, g[e] * w[k][e], -c * h[e]);
+                if (a.gh) {
+                    load_vec<T, VEC>(row + 2 * a.dim + i, h);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) g[e] += h[e];
+                }
+                store_vec<T, VEC>(static_cast<T*>(a.gx) + r * a.dim + i, g);
+            }
+        }
+    }
+    if (!a.partial) return;
+    float* dst = a.partial + static_cast<int64_t>(blockIdx.x) * a.dim;
+#pragma unroll
+    for (int k = 0; k < KV; ++k) {
+        const int i = (k * kThreads + t) * VEC;
+        if (i < a.dim) {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 4)
+                *reinterpret_cast<float4*>(dst + i + e) = make_float4(acc[k][e], acc[k][e + 1], acc[k][e + 2], acc[k][e + 3]);
+        }
+    }
+}
+
 // gw[c] = sum of the partial rows; 32 columns a CTA, 8 threads a column
 template <typename T>
 __global__ void __launch_bounds__(256) rms_gw_kernel(const float* __restrict__ partial, int rows, int dim,
@@ -369,9 +479,8 @@ cudaError_t by_width(int elems, Fn&& fn) {
     return cudaErrorInvalidValue;
 }
 
-// The backward keeps its part of gw besides three rows' vectors: at most two vectors a thread, which leaves
-// registers for 1024 threads an SM.
-template <int VEC, typename Fn>
+// Rows that the ring does not take: of up to two vectors a thread of a warp, unaligned ones, and long fp32 ones.
+template <typename T, int VEC, typename Fn>
 cudaError_t by_width_bwd(int elems, Fn&& fn) {
     auto go = [&](auto g, auto kv) { return fn(g, kv); };
 #define MMLTK_RMS_WIDTH(G, KV) \
@@ -383,12 +492,7 @@ cudaError_t by_width_bwd(int elems, Fn&& fn) {
     } else {
         MMLTK_RMS_WIDTH(32, 1);
         MMLTK_RMS_WIDTH(32, 2);
-        MMLTK_RMS_WIDTH(128, 1);
-        MMLTK_RMS_WIDTH(128, 2);
-        MMLTK_RMS_WIDTH(256, 2);
-        MMLTK_RMS_WIDTH(512, 2);
-        MMLTK_RMS_WIDTH(1024, 2);
-        if constexpr (VEC == 4) MMLTK_RMS_WIDTH(1024, 4);
+        if constexpr (sizeof(T) == 4) MMLTK_RMS_WIDTH(1024, 4);
     }
 #undef MMLTK_RMS_WIDTH
     return cudaErrorInvalidValue;
@@ -437,6 +541,42 @@ int bwd_blocks(int64_t rows, int group) {
 }
 }  // namespace
 
+namespace {
+template <typename T>
+cudaError_t sum_gw(const RmsBwdArgs& a, int blocks, cudaStream_t st) {
+    if (!a.partial) return cudaSuccess;
+    rms_gw_kernel<T><<<(a.dim + 31) / 32, 256, 0, st>>>(a.partial, blocks, a.dim, a.gw, a.w_f32);
+    return cudaGetLastError();
+}
+
+// Rows of more than a warp's registers, 16-byte aligned.  As many CTAs an SM as keep three stages (two from 24 KB a
+// stage on): the barriers of one row are then under other rows' loads (16384 x 8192: 171 us with two CTAs of two
+// stages, 189 with one of four; 65536 x 1024: 101 with eight CTAs, 123 with four).
+template <typename T>
+cudaError_t ring_bwd(const RmsBwdArgs& a, cudaStream_t st) {
+    const int vecs = a.dim / VecOf<T>::kN;
+    if (vecs <= 64) return cudaErrorNotSupported;
+    const int stage = 3 * a.dim * static_cast<int>(sizeof(T));
+    const int per_sm = vecs <= 128 ? 8 : (vecs <= 256 ? 6 : (3 * stage <= 72 * 1024 ? 3 : (2 * stage <= 108 * 1024 ? 2 : 1)));
+    const int stages = std::min(kRingStages, 216 * 1024 / per_sm / stage);
+    if (stages < 2) return cudaErrorNotSupported;
+    const int blocks = static_cast<int>(std::min<int64_t>(a.rows, static_cast<int64_t>(num_sms()) * per_sm));
+    auto run = [&](auto kern, int threads) -> cudaError_t {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, stages * stage);
+        if (e != cudaSuccess) return e;
+        kern<<<blocks, threads, stages * stage, st>>>(a, stages);
+        e = cudaGetLastError();
+        return e != cudaSuccess ? e : sum_gw<T>(a, blocks, st);
+    };
+    if (vecs <= 128) return run(rms_bwd_ring_kernel<T, 128, 1>, 128);
+    if (vecs <= 256) return run(rms_bwd_ring_kernel<T, 128, 2>, 128);
+    if (vecs <= 512) return run(rms_bwd_ring_kernel<T, 256, 2>, 256);
+    if (vecs <= 1024) return run(rms_bwd_ring_kernel<T, 256, 4>, 256);
+    if (vecs <= 2048) return run(rms_bwd_ring_kernel<T, 512, 4>, 512);
+    return cudaErrorNotSupported;      // fp32 rows of over 8192 elements: two stages would not fit
+}
+}  // namespace
+
 int rms_bwd_partials(Elt, int64_t rows, int) {
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, num_sms() * 8)));
 }
@@ -449,16 +589,18 @@ cudaError_t launch_rms_bwd(Elt et, const RmsBwdArgs& a, cudaStream_t st) {
         const bool vec = a.dim % kN == 0 && aligned(a.h) && a.ldh % kN == 0 && aligned(a.w) &&
                          a.ldgy % kN == 0 && aligned(a.gy) &&
                          (!a.gh || (a.ldgh % kN == 0 && aligned(a.gh)));
+        if (vec && a.rows > 0) {
+            const cudaError_t e = ring_bwd<T>(a, st);
+            if (e != cudaErrorNotSupported) return e;
+        }
         auto run = [&](auto vc) -> cudaError_t {
             constexpr int VEC = decltype(vc)::value;
-            return by_width_bwd<VEC>(a.dim, [&](auto gc, auto kc) -> cudaError_t {
+            return by_width_bwd<T, VEC>(a.dim, [&](auto gc, auto kc) -> cudaError_t {
                 constexpr int G = decltype(gc)::value, KV = decltype(kc)::value;
                 const int blocks = bwd_blocks(a.rows, G);
                 rms_bwd_kernel<T, VEC, G, KV><<<blocks, G == 32 ? 256 : G, 0, st>>>(a);
-                cudaError_t e = cudaGetLastError();
-                if (e != cudaSuccess || !a.partial) return e;
-                rms_gw_kernel<T><<<(a.dim + 31) / 32, 256, 0, st>>>(a.partial, blocks, a.dim, a.gw, a.w_f32);
-                return cudaGetLastError();
+                const cudaError_t e = cudaGetLastError();
+                return e != cudaSuccess ? e : sum_gw<T>(a, blocks, st);
             });
         };
         if (vec) return run(std::integral_constant<int, kN>{});
