@@ -1,0 +1,60 @@
+"""A pre-norm MLP block on the RMS norm, and its low-precision serving form.
+
+``PreNormMlp``            h = x + residual; y = fc2(GELU(fc1(rms_norm(h)))); returns (y, h) -- y is the next
+                          block's x, h its residual.  Trainable.
+``PreNormMlp.quantize``   the same block with 8- or 4-bit weights: three kernels for norm + fc1 + fc2 in mxfp8
+                          (the norm and fc1 write the next product's 8-bit input), no gradient.
+
+No counterpart in the reference, whose blocks use LayerNorm and 16-bit linears.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+import torch.nn as nn
+
+from .. import ops
+
+__all__ = ["PreNormMlp", "QuantizedPreNormMlp"]
+
+
+class PreNormMlp(nn.Module):
+    def __init__(self, dim: int, hidden: int, eps: float = 1e-6):
+        super().__init__()
+        self.norm_weight = nn.Parameter(torch.ones(dim))
+        self.fc1, self.fc2 = nn.Linear(dim, hidden), nn.Linear(hidden, dim)
+        self.eps = eps
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        if residual is None:
+            n, h = ops.rms_norm(x, self.norm_weight, self.eps), x
+        else:
+            n, h = ops.add_rms_norm(x, residual, self.norm_weight, self.eps)
+        n = ops.linear(n, self.fc1.weight, self.fc1.bias, act="gelu")
+        return ops.linear(n, self.fc2.weight, self.fc2.bias), h
+
+    @torch.no_grad()
+    def quantize(self, fmt: str = "mxfp8") -> "QuantizedPreNormMlp":
+        return QuantizedPreNormMlp(self.norm_weight.detach(), ops.mx_quantize(self.fc1.weight, fmt), self.fc1.bias,
+                                   ops.mx_quantize(self.fc2.weight, fmt), self.fc2.bias, self.eps)
+
+
+class QuantizedPreNormMlp:
+    """Weights as ``MXTensor``; ``block(x, residual)`` as ``PreNormMlp``, from one token to long batches."""
+
+    def __init__(self, norm_weight, w1: ops.MXTensor, b1, w2: ops.MXTensor, b2, eps: float = 1e-6):
+        if w1.fmt != w2.fmt or w1.shape[0] != w2.shape[1]:
+            raise ValueError(f"weights {w1} and {w2} do not make an MLP")
+        self.norm_weight, self.w1, self.w2, self.eps = norm_weight, w1, w2, eps
+        self.b1, self.b2 = (None if b is None else b.detach() for b in (b1, b2))
+
+    @torch.no_grad()
+    def __call__(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        fmt = self.w1.fmt
+        n, h = ops.rms_norm_quantized(x, self.norm_weight, self.eps, residual=residual, fmt=fmt)
+        if fmt == "mxfp8":      # the hidden activations leave the first product in the second one's format
+            n = ops.mx_linear(n, self.w1, self.b1, act="gelu", out_fmt=fmt)
+        else:
+            n = ops.mx_linear(n, self.w1, self.b1, act="gelu", out_dtype=x.dtype)
+        return ops.mx_linear(n, self.w2, self.b2, out_dtype=x.dtype), h

@@ -5,6 +5,7 @@ library baseline of the same op, timed with CUDA events after warm-up.
     python -m mmltk_b200.ops.bench_ops msda      # MSDeformAttn fwd+bwd vs fp32 reference path
     python -m mmltk_b200.ops.bench_ops attn      # attention fwd+bwd of the RF-DETR-M shapes per SDPA backend
     python -m mmltk_b200.ops.bench_ops kernels   # LayerNorm, criterion (matcher + solver + losses), post-process
+    python -m mmltk_b200.ops.bench_ops lowp      # RMS norm, microscaled formats and products, the pre-norm MLP block
 
 Inputs are larger than L2 where the op allows; each timing is the median of
 several event-timed runs.
@@ -17,7 +18,7 @@ import statistics
 
 import torch
 
-__all__ = ["time_ms", "time_graph_ms", "bench_gemm", "bench_msda", "bench_attn"]
+__all__ = ["time_ms", "time_graph_ms", "bench_gemm", "bench_msda", "bench_attn", "bench_lowp"]
 
 
 def time_ms(fn, warmup: int = 5, iters: int = 20, reps: int = 5) -> float:
@@ -427,9 +428,64 @@ def bench_kernels(device="cuda", quick=False):
     return rows
 
 
+def bench_lowp(device="cuda", quick=False):
+    """RMS norm, microscaled quantisation and products, and the pre-norm MLP block, from CUDA-graph replays:
+    us, and the bytes and operations that a call cannot do without per second."""
+    from . import MXTensor, add_rms_norm, mx_linear, mx_quantize, rms_norm_quantized
+    from ..models.prenorm_mlp import PreNormMlp
+    rows = []
+
+    def add(name, fn, bytes_=0.0, flops=0.0):
+        if quick:
+            for _ in range(3):
+                fn()
+            torch.cuda.synchronize()
+            return
+        us = time_graph_ms(fn, iters=10) * 1e3
+        rows.append({"op": name, "us": round(us, 2), "gbs": round(bytes_ / us / 1e3, 1),
+                     "tflops": round(flops / us / 1e6, 1)})
+
+    def normal(*shape):
+        return torch.randn(*shape, device=device).bfloat16()
+
+    with torch.no_grad():
+        for m, d in ((1, 2048), (10400, 384), (32768, 4096)):
+            x, r, w = normal(m, d), normal(m, d), normal(d)
+            add(f"add_rms_norm {m}x{d}", lambda: add_rms_norm(x, r, w), 8.0 * m * d)
+            add(f"rms_norm_quantized mxfp8 {m}x{d}", lambda: rms_norm_quantized(x, w, residual=r), 7.03 * m * d)
+        for m, d in ((1536, 384), (16384, 8192)):
+            x = normal(m, d)
+            for fmt, out in (("mxfp4", 0.53), ("nvfp4", 0.56), ("mxfp8", 1.03)):
+                add(f"mx_quantize {fmt} {m}x{d}", lambda: mx_quantize(x, fmt), (2 + out) * m * d)
+                t = mx_quantize(x, fmt)
+                add(f"dequantize {fmt} {m}x{d}", t.dequantize, (2 + out) * m * d)
+        for fmt, m, n, k, act, out in (("nvfp4", 1, 4096, 4096, None, None), ("mxfp8", 1, 8192, 8192, None, None),
+                                       ("mxfp8", 17, 2050, 1000, None, None), ("nvfp4", 128, 4096, 4096, None, None),
+                                       ("mxfp4", 10400, 1536, 384, "gelu", None),
+                                       ("mxfp8", 31200, 2048, 256, "relu", "mxfp8"),
+                                       ("mxfp4", 8192, 8192, 8192, None, None), ("nvfp4", 8192, 8192, 8192, None, None),
+                                       ("mxfp8", 8192, 8192, 8192, None, None)):
+            x, wq, b = normal(m, k), mx_quantize(normal(n, k), fmt), normal(n)
+            one = torch.ones(1, device=device) if fmt == "nvfp4" else None
+            xq = mx_quantize(x, fmt, one)
+            size = n * k * {"mxfp4": 0.53125, "nvfp4": 0.5625, "mxfp8": 1.03125}[fmt] + m * n * (1.03 if out else 2)
+            for name, inp in (("16-bit x", x), ("quantised x", xq)):
+                extra = 2.0 * m * k if not isinstance(inp, MXTensor) else xq.codes.nbytes
+                add(f"mx_linear {fmt} {m}x{n}x{k} {act or ''} {name}{' -> ' + out if out else ''}",
+                    lambda: mx_linear(inp, wq, b, act=act, out_fmt=out), size + extra, 2.0 * m * n * k)
+        block = PreNormMlp(384, 1536).to(device, torch.bfloat16)
+        for m in (1, 1300, 10400):
+            x, r = normal(m, 384), normal(m, 384)
+            add(f"pre-norm MLP 384-1536 bf16, {m} rows", lambda: block(x, r), flops=4.0 * m * 384 * 1536)
+            for fmt in ("mxfp8", "mxfp4"):
+                q = block.quantize(fmt)
+                add(f"pre-norm MLP 384-1536 {fmt}, {m} rows", lambda: q(x, r), flops=4.0 * m * 384 * 1536)
+    return rows
+
+
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("what", choices=["gemm", "msda", "attn", "kernels"])
+    ap.add_argument("what", choices=["gemm", "msda", "attn", "kernels", "lowp"])
     ap.add_argument("--shape", default=None, help="run one GEMM shape (see GEMM_SHAPES)")
     ap.add_argument("--quick", nargs="?", const="default", default=None,
                     help="launch a few times without timing (profiler runs); attn: '--quick short' runs the "
@@ -445,6 +501,8 @@ def main():
         rows = bench_msda(quick=bool(args.quick))
     elif args.what == "kernels":
         rows = bench_kernels(quick=bool(args.quick))
+    elif args.what == "lowp":
+        rows = bench_lowp(quick=bool(args.quick))
     else:
         rows = bench_attn(quick=args.quick)
     for r in rows:

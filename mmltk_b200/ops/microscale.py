@@ -38,6 +38,16 @@ from ._ext import kernels
 __all__ = ["MXTensor", "mx_quantize", "mx_linear", "mx_status", "format_id", "quantize_reference",
            "dequantize_reference"]
 
+_ext = []
+
+
+def _kernels():
+    """The kernel extension, looked up once: the lookup reads the environment, a tenth of a small call's time."""
+    if not _ext:
+        _ext.append(kernels())
+    return _ext[0]
+
+
 _FORMATS = {"mxfp4": 0, "nvfp4": 1, "mxfp8": 2}
 _BLOCK = {"mxfp4": 32, "nvfp4": 16, "mxfp8": 32}
 _BITS = {"mxfp4": 4, "nvfp4": 4, "mxfp8": 8}
@@ -81,11 +91,11 @@ class MXTensor:
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values, rounded once to ``dtype`` (bf16, fp16 or fp32)."""
         if self.codes.is_cuda:
-            y = kernels().mx_dequantize(self.codes, self.scales, self.global_scale, _FORMATS[self.fmt], self.rows,
-                                        self.shape[-1], dtype)
+            y = _kernels().mx_dequantize(self.codes, self.scales, self.global_scale, _FORMATS[self.fmt], self.rows,
+                                         self.shape[-1], dtype)
         else:
             y = dequantize_reference(self).to(dtype)
-        return y.view(self.shape)
+        return y if len(self.shape) == 2 else y.view(self.shape)
 
     def __repr__(self) -> str:
         return f"MXTensor({self.fmt}, shape={self.shape}, device={self.device})"
@@ -96,7 +106,7 @@ def mx_quantize(x: torch.Tensor, fmt: str, global_scale: Optional[torch.Tensor] 
     tensor scale to use; by default it is found from x (one more pass over it)."""
     f = format_id(fmt)
     if x.is_cuda:
-        codes, scales, g = kernels().mx_quantize(x, f, global_scale)
+        codes, scales, g = _kernels().mx_quantize(x, f, global_scale)
         return MXTensor(codes, scales, fmt, x.shape, g)
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("mx_quantize: needs a last dimension of at least one element")
@@ -149,13 +159,15 @@ def mx_linear(x, weight: MXTensor, bias: Optional[torch.Tensor] = None, *, act: 
     shape = (*x.shape[:-1], n)
     if weight.codes.is_cuda:
         if quantised:
-            out = kernels().mx_linear(None, x.codes, x.scales, x.global_scale, x.rows, weight.codes, weight.scales,
-                                      weight.global_scale, _FORMATS[fmt], n, k, bias, _ACTS[act], out_dtype,
-                                      out_fmt is not None)
+            out = _kernels().mx_linear(None, x.codes, x.scales, x.global_scale, x.rows, weight.codes, weight.scales,
+                                       weight.global_scale, _FORMATS[fmt], n, k, bias, _ACTS[act], out_dtype,
+                                       out_fmt is not None)
         else:
-            out = kernels().mx_linear(x, None, None, act_scale, 0, weight.codes, weight.scales, weight.global_scale,
-                                      _FORMATS[fmt], n, k, bias, _ACTS[act], out_dtype, out_fmt is not None)
-        return out[0].view(shape) if out_fmt is None else MXTensor(out[0], out[1], out_fmt, shape)
+            out = _kernels().mx_linear(x, None, None, act_scale, 0, weight.codes, weight.scales, weight.global_scale,
+                                       _FORMATS[fmt], n, k, bias, _ACTS[act], out_dtype, out_fmt is not None)
+        if out_fmt is not None:
+            return MXTensor(out[0], out[1], out_fmt, shape)
+        return out[0] if len(shape) == 2 else out[0].view(shape)
     if not quantised:
         if x.shape[-1] != k:
             raise ValueError(f"mx_linear: input [..., {k}] expected, got {tuple(x.shape)}")
@@ -173,7 +185,7 @@ def mx_linear(x, weight: MXTensor, bias: Optional[torch.Tensor] = None, *, act: 
 def mx_status(device=None) -> int:
     """Non-zero when a product on ``device`` gave up a bounded wait since the last call (its output is then invalid)."""
     dev = torch.device("cuda" if device is None else device)
-    return kernels().mx_status(torch.cuda.current_device() if dev.index is None else dev.index)
+    return _kernels().mx_status(torch.cuda.current_device() if dev.index is None else dev.index)
 
 
 # ---------------------------------------------------------------- the plain definition

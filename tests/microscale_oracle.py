@@ -55,10 +55,11 @@ def quantize(x, fmt, g=None):
             byte[bad, b] = 0x7F
         else:
             top = GRID[bits][-1]
-            p = np.full(rows, -127)
-            for r in range(rows):
-                while p[r] < 127 and am[r] > top * 2.0 ** int(p[r]):
-                    p[r] += 1
+            e = np.frexp(am)[1]                                  # am < 2^e: the answer is one of three
+            p = np.clip(e - (3 if bits == 4 else 9), -127, 127)
+            for _ in range(2):
+                p = np.where((p < 127) & (am > top * 2.0 ** p.astype(np.float64)), p + 1, p)
+            p = np.where(am > 0, p, -127)
             scale = 2.0 ** p.astype(np.float64)
             q = np.where(bad[:, None], 0, xb) / scale[:, None]
             byte[:, b] = np.where(bad, 255, p + 127)
