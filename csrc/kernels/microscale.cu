@@ -87,45 +87,42 @@ __global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 4 : 3)
     }
 }
 
-// largest magnitude of a matrix, as bits (an order that keeps NaN); max does not depend on the order
+template <typename T>
+__device__ __forceinline__ uint32_t amax_bits_of(const uint4& w) {
+    float f[VecOf<T>::kN];
+    unpack16(w, f, T());
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < VecOf<T>::kN; ++e) m = max(m, abs_bits(f[e]));
+    return m;
+}
+
+// Largest magnitude of a matrix, as bits (an order that keeps NaN; max does not depend on the order).  A dense one is
+// read as one row.
 template <typename T>
 __global__ void __launch_bounds__(512) mx_amax_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t dim,
-                                                      uint32_t* __restrict__ amax, bool vec) {
+                                                      uint32_t* __restrict__ amax) {
     constexpr int kN = VecOf<T>::kN;
     uint32_t m = 0;
     allow_next();
-    if (vec) {   // whole 16-byte vectors: pitch, base and width all multiples
-        const int64_t per_row = dim / kN, total = rows * per_row;
-        const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+    // CTAs side by side in a row, then over the rows
+    const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+        const T* row = x + r * ld;
         int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-        const bool dense = ld == dim;
-        for (; i + 3 * step < total; i += 4 * step) {
+        const bool aligned = reinterpret_cast<uintptr_t>(row) % 16 == 0;
+        const int64_t whole = aligned ? dim / kN : 0, total = (dim + kN - 1) / kN;
+        for (; i + 3 * step < whole; i += 4 * step) {
             uint4 w[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int64_t j = i + u * step;
-                w[u] = dense ? reinterpret_cast<const uint4*>(x)[j]
-                             : reinterpret_cast<const uint4*>(x + (j / per_row) * ld)[j % per_row];
-            }
+            for (int u = 0; u < 4; ++u) w[u] = reinterpret_cast<const uint4*>(row)[i + u * step];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                float f[kN];
-                unpack16(w[u], f, T());
-#pragma unroll
-                for (int e = 0; e < kN; ++e) m = max(m, abs_bits(f[e]));
-            }
+            for (int u = 0; u < 4; ++u) m = max(m, amax_bits_of<T>(w[u]));
         }
         for (; i < total; i += step) {
-            float f[kN];
-            unpack16(reinterpret_cast<const uint4*>(x + (i / per_row) * ld)[i % per_row], f, T());
-#pragma unroll
-            for (int e = 0; e < kN; ++e) m = max(m, abs_bits(f[e]));
+            const int64_t left = dim - i * kN;
+            m = max(m, amax_bits_of<T>(load_any(row + i * kN, left < kN ? static_cast<int>(left) : kN)));
         }
-    } else {
-        const int64_t total = rows * dim;
-        for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-             i += static_cast<int64_t>(gridDim.x) * blockDim.x)
-            m = max(m, abs_bits(to_f(x[(i / dim) * ld + i % dim])));
     }
     m = __reduce_max_sync(0xffffffffu, m);
     if ((threadIdx.x & 31) == 0 && m) atomicMax(amax, m);
@@ -178,9 +175,9 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __res
 #pragma unroll
             for (int e = 0; e < 16; e += kN) *reinterpret_cast<uint4*>(o + e) = pack16(v + e, T());
         } else {
+            const int n = static_cast<int>(dim - col < 16 ? dim - col : 16);
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (col + e < dim) o[e] = from_f<T>(v[e]);
+            for (int e = 0; e < 16; e += kN) store_any_vec(o + e, pack16(v + e, T()), n - e);
         }
     }
 }
@@ -209,10 +206,11 @@ cudaError_t launch_mx_quantize(Elt et, MxFormat f, const void* x, int64_t ld, in
         if (f == MxFormat::kNvFp4 && amax) {
             cudaError_t e = cudaMemsetAsync(amax, 0, sizeof(uint32_t), st);
             if (e != cudaSuccess) return e;
-            const int64_t work = (rows * dim + 512 * kN * 4 - 1) / (512 * kN * 4);
-            const int blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(work, num_sms() * 4)));
-            mx_amax_kernel<T><<<blocks, 512, 0, st>>>(static_cast<const T*>(x), ld, rows, dim, amax,
-                                                      align && dim % kN == 0);
+            const int64_t r = ld == dim ? 1 : rows, d = ld == dim ? rows * dim : dim;
+            const int64_t across = std::max<int64_t>(1, std::min<int64_t>((d + 512 * kN - 1) / (512 * kN), num_sms() * 4));
+            const dim3 grid(static_cast<unsigned>(across),
+                            static_cast<unsigned>(std::min<int64_t>(r, std::max<int64_t>(1, num_sms() * 4 / across))));
+            mx_amax_kernel<T><<<grid, 512, 0, st>>>(static_cast<const T*>(x), ld, r, d, amax);
             e = cudaGetLastError();
             if (e != cudaSuccess) return e;
         }

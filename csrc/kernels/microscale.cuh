@@ -225,6 +225,82 @@ __device__ __forceinline__ void st_global_32(void* p, const uint4& a, const uint
                  : "memory");
 }
 
+// ---------------------------------------------------------------- vectors at any element's address
+// Bytes sh .. sh + 15 of the 32 in a, b.
+__device__ __forceinline__ uint4 shift16(const uint4& a, const uint4& b, uint32_t sh) {
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (sh & 8) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (sh & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    const uint32_t bits = (sh & 3) * 8;
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                      __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+// The 16 bytes of elements at p, of which the first n are read and the rest zero (n <= 0: none).  One or two aligned
+// loads of 16-byte granules that hold at least one of the n, so nothing outside the allocation's granules is read.
+template <typename T>
+__device__ __forceinline__ uint4 load_any(const T* p, int n) {
+    constexpr int kN = 16 / sizeof(T);
+    if (n <= 0) return make_uint4(0, 0, 0, 0);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p), base = at & ~uintptr_t(15);
+    const uint32_t sh = static_cast<uint32_t>(at & 15);
+    const uint4 a = *reinterpret_cast<const uint4*>(base);
+    uint4 w = a;
+    if (sh) {
+        uint4 b = make_uint4(0, 0, 0, 0);
+        if (base + 16 < at + n * sizeof(T)) b = *reinterpret_cast<const uint4*>(base + 16);
+        w = shift16(a, b, sh);
+    }
+    if (n < kN) {      // zero the rest
+        uint32_t* u = &w.x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int have = (n * static_cast<int>(sizeof(T)) - 4 * i) * 8;      // valid bits of this word
+            u[i] = have >= 32 ? u[i] : (have <= 0 ? 0u : u[i] & (0xffffffffu >> (32 - have)));
+        }
+    }
+    return w;
+}
+// Stores the first n elements of w at p, in the widest pieces that p's address allows.
+template <typename T>
+__device__ __forceinline__ void store_any_vec(T* p, const uint4& w, int n) {
+    constexpr int kN = 16 / sizeof(T);
+    const uint32_t sh = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15);
+    if (n >= kN && sh == 0) {
+        *reinterpret_cast<uint4*>(p) = w;
+    } else if (n >= kN && (sh & 7) == 0) {
+        reinterpret_cast<uint2*>(p)[0] = make_uint2(w.x, w.y);
+        reinterpret_cast<uint2*>(p)[1] = make_uint2(w.z, w.w);
+    } else if (n >= kN && (sh & 3) == 0) {
+        uint32_t* q = reinterpret_cast<uint32_t*>(p);
+        q[0] = w.x;
+        q[1] = w.y;
+        q[2] = w.z;
+        q[3] = w.w;
+    } else if (n >= kN) {      // 16-bit elements at an odd one: half a word, three words, half a word
+        unsigned short* h = reinterpret_cast<unsigned short*>(p);
+        uint32_t* q = reinterpret_cast<uint32_t*>(h + 1);
+        h[0] = static_cast<unsigned short>(w.x);
+        q[0] = __funnelshift_r(w.x, w.y, 16);
+        q[1] = __funnelshift_r(w.y, w.z, 16);
+        q[2] = __funnelshift_r(w.z, w.w, 16);
+        h[7] = static_cast<unsigned short>(w.w >> 16);
+    } else {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            if (i < n) {
+                if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[i] = u[i];
+                else reinterpret_cast<unsigned short*>(p)[i] = static_cast<unsigned short>(u[i >> 1] >> (16 * (i & 1)));
+            }
+    }
+}
+
 // Lets a kernel use `bytes` of dynamic shared memory; asked of each device once (a launch's host time counts).
 template <typename Kern>
 cudaError_t allow_smem(Kern kern, std::atomic<uint64_t>& done, int bytes) {
@@ -261,11 +337,9 @@ struct Raw16 {
 #pragma unroll
             for (int i = 0; i < kVecs; ++i) w[i] = reinterpret_cast<const uint4*>(x + col)[i];
         } else {
-            float f[16];
+            const int n = static_cast<int>(dim - col < 16 ? dim - col : 16);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) f[i] = col + i < dim ? to_f(x[col + i]) : 0.f;
-#pragma unroll
-            for (int i = 0; i < kVecs; ++i) w[i] = pack16(f + i * VecOf<T>::kN, T());     // exact: values of type T
+            for (int i = 0; i < kVecs; ++i) w[i] = load_any(x + col + i * VecOf<T>::kN, n - i * VecOf<T>::kN);
         }
     }
     __device__ __forceinline__ void get(float* v) const {

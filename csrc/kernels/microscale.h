@@ -30,7 +30,7 @@ constexpr int kRmsMaxDim = 16384;
 struct RmsFwdArgs {
     const void* x;
     const void* res;      // optional: the norm reads round(x + res), stored to h
-    const void* w;        // [dim], x's type or fp32
+    const void* w;        // [dim], x's type or fp32, 16-byte aligned
     void* y;              // [rows, dim] of x's type (contiguous), or null with codes
     void* h;              // [rows, dim], with res
     float* rstd;          // optional [rows]
@@ -53,13 +53,14 @@ struct RmsBwdArgs {
     const float* rstd;
     void* gx;
     void* gw;             // [dim] of w's type
-    float* partial;       // [rms_bwd_partials(...), dim] work space, null: no gw
+    float* partial;       // [rms_bwd_partials(rows), rms_partial_pitch(dim)] work space, null: no gw
     int* status;          // set when a bounded wait gave up
     int64_t rows, ldgy, ldgh, ldh;
     int dim;
     bool w_f32;
 };
-int rms_bwd_partials(Elt et, int64_t rows, int dim);
+constexpr int rms_partial_pitch(int dim) { return (dim + 7) / 8 * 8; }
+int rms_bwd_partials(int64_t rows);
 cudaError_t launch_rms_bwd(Elt et, const RmsBwdArgs& a, cudaStream_t st);
 
 // ---------------------------------------------------------------- product

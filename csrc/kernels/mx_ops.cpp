@@ -159,13 +159,18 @@ void check_norm(const torch::Tensor& x, const torch::Tensor& w, const OptTensor&
                     what, ": residual must match the input's shape, dtype and device");
 }
 
+torch::Tensor aligned_weight(const torch::Tensor& w) {      // vector loads
+    torch::Tensor c = w.contiguous();
+    return aligned16(c) ? c : c.clone();
+}
+
 struct NormOut {
     torch::Tensor y, h, rstd, codes, scales;
 };
 NormOut norm_forward(const torch::Tensor& x, const torch::Tensor& w_in, const OptTensor& res, double eps, bool want_rstd,
                      const MxFormat* fmt, const float* g, const char* what) {
     at::cuda::CUDAGuard guard(x.device());
-    const torch::Tensor xr = as_rows(x), w = w_in.contiguous();
+    const torch::Tensor xr = as_rows(x), w = aligned_weight(w_in);
     NormOut o;
     RmsFwdArgs a{};
     a.rows = xr.size(0);
@@ -207,7 +212,7 @@ std::pair<torch::Tensor, torch::Tensor> norm_backward(const torch::Tensor& gy, c
                                                       const torch::Tensor& h, const torch::Tensor& w_in,
                                                       const torch::Tensor& rstd, bool want_gw) {
     at::cuda::CUDAGuard guard(h.device());
-    const torch::Tensor hr = as_rows(h), w = w_in.contiguous();
+    const torch::Tensor hr = as_rows(h), w = aligned_weight(w_in);
     RmsBwdArgs a{};
     a.rows = hr.size(0);
     a.dim = static_cast<int>(hr.size(1));
@@ -233,7 +238,7 @@ std::pair<torch::Tensor, torch::Tensor> norm_backward(const torch::Tensor& gy, c
     if (want_gw) {
         gw = torch::empty(w.sizes(), w.options());
         a.gw = gw.data_ptr();
-        partial = torch::empty({rms_bwd_partials(et, a.rows, a.dim), a.dim}, h.options().dtype(torch::kFloat32));
+        partial = torch::empty({rms_bwd_partials(a.rows), rms_partial_pitch(a.dim)}, h.options().dtype(torch::kFloat32));
         a.partial = partial.data_ptr<float>();
     }
     check_cuda(launch_rms_bwd(et, a, cur_stream()), "rms_norm backward");

@@ -8,9 +8,8 @@
 //
 // Memory-bound.  A row is held in registers by a group of threads -- a warp up to 1024 16-bit
 // elements, a CTA of 128 to 512 threads beyond -- so every element is read once; statistics are
-// fp32.  A thread's elements are 16-byte vectors kGroup vectors apart (VEC = 1 where the width,
-// the pitch or an address is not a multiple of 16 bytes), so the 4 or 8 threads of a scale block
-// are neighbours in a warp and find its maximum with two or three shuffles.
+// fp32.  A thread's elements are 16-byte vectors kGroup vectors apart, so the 2 to 8 threads of a
+// scale block are neighbours in a warp and find its maximum with at most three shuffles.
 #include "microscale.cuh"
 #include "tcgen05.cuh"
 
@@ -22,59 +21,46 @@ using namespace mx;
 
 constexpr int kRingStages = 8;
 
-template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T* p, float* f) {
-    if constexpr (VEC == 1) {
-        f[0] = to_f(*p);
-    } else {
-        unpack16(*reinterpret_cast<const uint4*>(p), f, T());
-    }
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void store_vec(T* p, const float* f) {
-    if constexpr (VEC == 1) {
-        *p = from_f<T>(f[0]);
-    } else {
-        *reinterpret_cast<uint4*>(p) = pack16(f, T());
-    }
-}
 // A vector of a row as loaded: unpacked where it is used, so that a waiting row takes 4 registers per 16 bytes
-// (8 as fp32), which is what decides how many rows an SM has in flight.
-template <typename T, int VEC>
+// (8 as fp32), which is what decides how many rows an SM has in flight.  `left`: elements of the row from here on.
+// Rows that start anywhere (kAligned = false: a width or pitch that is no multiple of 16 bytes) are read in
+// aligned granules and shifted, and written in the widest pieces the address allows.
+template <typename T, bool kAligned>
 struct Raw {
     uint4 w;
-    __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const uint4*>(p); }
-    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = w; }
+    __device__ __forceinline__ void load(const T* p, int left) {
+        if constexpr (kAligned) w = *reinterpret_cast<const uint4*>(p);
+        else w = load_any(p, min(left, VecOf<T>::kN));
+    }
+    __device__ __forceinline__ void store(T* p, int left) const {
+        if constexpr (kAligned) *reinterpret_cast<uint4*>(p) = w;
+        else store_any_vec(p, w, min(left, VecOf<T>::kN));
+    }
     __device__ __forceinline__ void get(float* f) const { unpack16(w, f, T()); }
     __device__ __forceinline__ void set(const float* f) { w = pack16(f, T()); }
     __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
 };
-template <typename T>
-struct Raw<T, 1> {
-    T v;
-    __device__ __forceinline__ void load(const T* p) { v = *p; }
-    __device__ __forceinline__ void store(T* p) const { *p = v; }
-    __device__ __forceinline__ void get(float* f) const { f[0] = to_f(v); }
-    __device__ __forceinline__ void set(const float* f) { v = from_f<T>(f[0]); }
-    __device__ __forceinline__ void zero() { v = from_f<T>(0.f); }
-};
 
-// weights: x's type or fp32
-template <typename T, int VEC>
-__device__ __forceinline__ void load_w(const void* w, bool f32, int i, float* f) {
-    if (f32) {
-        const float* p = static_cast<const float*>(w) + i;
+// weights (16-byte aligned): x's type or fp32; zeros past the row
+template <typename T, bool kAligned>
+__device__ __forceinline__ void load_w(const void* w, bool f32, int i, int left, float* f) {
+    constexpr int kN = VecOf<T>::kN;
+    if (!kAligned && left < kN) {
 #pragma unroll
-        for (int e = 0; e < VEC; e += (VEC >= 4 ? 4 : 1)) {
-            if constexpr (VEC >= 4) {
-                const float4 t = *reinterpret_cast<const float4*>(p + e);
-                f[e] = t.x; f[e + 1] = t.y; f[e + 2] = t.z; f[e + 3] = t.w;
-            } else {
-                f[e] = p[e];
-            }
+        for (int e = 0; e < kN; ++e)
+            f[e] = e >= left ? 0.f : f32 ? static_cast<const float*>(w)[i + e] : to_f(static_cast<const T*>(w)[i + e]);
+    } else if (f32) {
+        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(w) + i);
+#pragma unroll
+        for (int e = 0; e < kN / 4; ++e) {
+            const float4 t = p[e];
+            f[4 * e] = t.x;
+            f[4 * e + 1] = t.y;
+            f[4 * e + 2] = t.z;
+            f[4 * e + 3] = t.w;
         }
     } else {
-        load_vec<T, VEC>(static_cast<const T*>(w) + i, f);
+        unpack16(*reinterpret_cast<const uint4*>(static_cast<const T*>(w) + i), f, T());
     }
 }
 
@@ -97,11 +83,11 @@ template <MxFormat F, int VEC>
 __device__ __forceinline__ void quantize_store(const float* v, int i, int64_t r, int64_t pitch, int kt, int span,
                                                uint8_t* codes, uint8_t* scales, float g) {
     using Tr = Traits<F>;
-    constexpr int kThreads = Tr::kBlock / VEC;      // threads of a block: 32 / 16, 8 / 4 or 4 / 2
-    float top = fabsf(v[0]);      // keeps a NaN
+    constexpr int kThreads = Tr::kBlock / VEC;      // threads of a block: 8 / 4 or 4 / 2
+    static_assert(4 * kThreads <= 32);
+    float top = 0.f;      // keeps a NaN
 #pragma unroll
-    for (int e = 1; e + 1 < VEC; e += 2) top = max3_abs_nan(top, v[e], v[e + 1]);
-    if constexpr (VEC % 2 == 0 && VEC > 1) top = max3_abs_nan(top, v[VEC - 1], v[VEC - 1]);
+    for (int e = 0; e < VEC; e += 2) top = max3_abs_nan(top, v[e], v[e + 1]);
     uint32_t m = abs_bits(top);
 #pragma unroll
     for (int o = 1; o < kThreads; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -110,42 +96,33 @@ __device__ __forceinline__ void quantize_store(const float* v, int i, int64_t r,
     uint8_t* row = codes + r * pitch;
     if constexpr (Tr::kBits == 8) {
         if (i < pitch) {
-            if constexpr (VEC == 8) {
+            if constexpr (VEC == 8)
                 *reinterpret_cast<uint2*>(row + i) = make_uint2(cvt_e4m3x4(v, sc.inv), cvt_e4m3x4(v + 4, sc.inv));
-            } else if constexpr (VEC == 4) {
+            else
                 *reinterpret_cast<uint32_t*>(row + i) = cvt_e4m3x4(v, sc.inv);
-            } else {
-                row[i] = static_cast<uint8_t>(cvt_e4m3x2(v[0] * sc.inv, 0.f));
-            }
         }
     } else {
-        if constexpr (VEC == 1) {
-            const float hi = __shfl_down_sync(0xffffffffu, v[0], 1);
-            if (i < 2 * pitch && (lane & 1) == 0) row[i >> 1] = static_cast<uint8_t>(cvt_e2m1x2(v[0] * sc.inv, hi * sc.inv));
-        } else if (i < 2 * pitch) {
+        if (i < 2 * pitch) {
             if constexpr (VEC == 8) {
                 *reinterpret_cast<uint32_t*>(row + (i >> 1)) = cvt_e2m1x8(v, sc.inv);
             } else {
-                *reinterpret_cast<uint16_t*>(row + (i >> 1)) = static_cast<uint16_t>(
-                    cvt_e2m1x2(v[0] * sc.inv, v[1] * sc.inv) | (cvt_e2m1x2(v[2] * sc.inv, v[3] * sc.inv) << 8));
+                const float2 a = scale2(v, sc.inv), b = scale2(v + 2, sc.inv);
+                *reinterpret_cast<uint16_t*>(row + (i >> 1)) =
+                    static_cast<uint16_t>(cvt_e2m1x2(a.x, a.y) | (cvt_e2m1x2(b.x, b.y) << 8));
             }
         }
     }
-    // the four scales of a tile's row, one 4-byte store, where a warp holds all four
-    if constexpr (4 * kThreads <= 32) {
-        uint32_t b = sc.byte;
-        b |= __shfl_down_sync(0xffffffffu, b, kThreads) << 8;
-        b |= __shfl_down_sync(0xffffffffu, b, 2 * kThreads) << 16;
-        if (i < span && (lane & (4 * kThreads - 1)) == 0)
-            *reinterpret_cast<uint32_t*>(scales + scale_offset(r, i / Tr::kBlock, kt)) = b;
-    } else {
-        if (i < span && (lane & (kThreads - 1)) == 0)
-            scales[scale_offset(r, i / Tr::kBlock, kt)] = static_cast<uint8_t>(sc.byte);
-    }
+    // the four scales of a tile's row, one 4-byte store
+    uint32_t b = sc.byte;
+    b |= __shfl_down_sync(0xffffffffu, b, kThreads) << 8;
+    b |= __shfl_down_sync(0xffffffffu, b, 2 * kThreads) << 16;
+    if (i < span && (lane & (4 * kThreads - 1)) == 0)
+        *reinterpret_cast<uint32_t*>(scales + scale_offset(r, i / Tr::kBlock, kt)) = b;
 }
 
-template <typename T, int VEC, int kGroup, int KV, bool kQuant>
+template <typename T, bool kAligned, int kGroup, int KV, bool kQuant>
 __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(RmsFwdArgs a) {
+    constexpr int VEC = VecOf<T>::kN;
     __shared__ float red[32];
     if (kQuant) allow_next();
     constexpr int kRows = kGroup == 32 ? 8 : 1;
@@ -160,21 +137,21 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(Rm
     }
     const T* xr = static_cast<const T*>(a.x) + r * a.ldx;
     const T* rr = a.res ? static_cast<const T*>(a.res) + r * a.ldr : nullptr;
-    Raw<T, VEC> v[KV];
+    Raw<T, kAligned> v[KV];
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
         const int i = (k * kGroup + t) * VEC;
-        if (i < a.dim) v[k].load(xr + i);
+        if (i < a.dim) v[k].load(xr + i, a.dim - i);
         else v[k].zero();
     }
     float s = 0.f;
     if (rr) {
         T* hr = static_cast<T*>(a.h) + r * a.dim;
-        Raw<T, VEC> u[KV];
+        Raw<T, kAligned> u[KV];
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
             const int i = (k * kGroup + t) * VEC;
-            if (i < a.dim) u[k].load(rr + i);
+            if (i < a.dim) u[k].load(rr + i, a.dim - i);
         }
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
@@ -187,7 +164,7 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(Rm
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) f[j] += e[j];
                 v[k].set(f);
-                v[k].store(hr + i);
+                v[k].store(hr + i, a.dim - i);
             }
         }
     }
@@ -211,10 +188,14 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(Rm
         v[k].get(f);
         if (i < a.dim) {
             float w[VEC];
-            load_w<T, VEC>(a.w, a.w_f32, i, w);
+            load_w<T, kAligned>(a.w, a.w_f32, i, a.dim - i, w);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) f[j] = f[j] * rstd * w[j];
-            if constexpr (!kQuant) store_vec<T, VEC>(static_cast<T*>(a.y) + r * a.dim + i, f);
+            if constexpr (!kQuant) {
+                Raw<T, kAligned> y;
+                y.set(f);
+                y.store(static_cast<T*>(a.y) + r * a.dim + i, a.dim - i);
+            }
         }
         if constexpr (kQuant) {
             if ((k * kGroup + (t & ~31)) * VEC >= span) continue;     // warp-uniform
@@ -234,9 +215,9 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(Rm
 // ---------------------------------------------------------------- backward
 // Persistent: a group of threads walks rows and keeps its columns' part of gw in registers; one partial
 // row per CTA, summed in a fixed order by rms_gw_kernel (no atomics: the same bits every run).
-template <typename T, int VEC, int kGroup, int KV>
-__global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 : (kGroup >= 512 ? 1024 / kGroup : 768 / kGroup))
-    rms_bwd_kernel(RmsBwdArgs a) {
+template <typename T, bool kAligned, int kGroup, int KV>
+__global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 : 1) rms_bwd_kernel(RmsBwdArgs a) {
+    constexpr int VEC = VecOf<T>::kN;
     constexpr int kRows = kGroup == 32 ? 8 : 1;
     __shared__ float red[2][32];
     __shared__ float part[kGroup == 32 ? 8 * 32 * VEC : 1];
@@ -252,14 +233,14 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + sub; r < a.rows;
          r += static_cast<int64_t>(gridDim.x) * kRows, turn ^= 1) {
         const float rstd = a.rstd[r];
-        Raw<T, VEC> hv[KV], gv[KV], ev[KV];
+        Raw<T, kAligned> hv[KV], gv[KV], ev[KV];
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
             const int i = (k * kGroup + t) * VEC;
             if (i < a.dim) {
-                hv[k].load(static_cast<const T*>(a.h) + r * a.ldh + i);
-                gv[k].load(static_cast<const T*>(a.gy) + r * a.ldgy + i);
-                if (a.gh) ev[k].load(static_cast<const T*>(a.gh) + r * a.ldgh + i);
+                hv[k].load(static_cast<const T*>(a.h) + r * a.ldh + i, a.dim - i);
+                gv[k].load(static_cast<const T*>(a.gy) + r * a.ldgy + i, a.dim - i);
+                if (a.gh) ev[k].load(static_cast<const T*>(a.gh) + r * a.ldgh + i, a.dim - i);
             }
         }
         float s = 0.f;
@@ -268,7 +249,7 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 
             const int i = (k * kGroup + t) * VEC;
             if (i < a.dim) {
                 float w[VEC], h[VEC], g[VEC];
-                load_w<T, VEC>(a.w, a.w_f32, i, w);
+                load_w<T, kAligned>(a.w, a.w_f32, i, a.dim - i, w);
                 hv[k].get(h);
                 gv[k].get(g);
 #pragma unroll
@@ -285,7 +266,7 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 
             const int i = (k * kGroup + t) * VEC;
             if (i < a.dim) {
                 float w[VEC], h[VEC], g[VEC];
-                load_w<T, VEC>(a.w, a.w_f32, i, w);
+                load_w<T, kAligned>(a.w, a.w_f32, i, a.dim - i, w);
                 hv[k].get(h);
                 gv[k].get(g);
 #pragma unroll
@@ -295,12 +276,13 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) g[e] += h[e];
                 }
-                store_vec<T, VEC>(static_cast<T*>(a.gx) + r * a.dim + i, g);
+                hv[k].set(g);
+                hv[k].store(static_cast<T*>(a.gx) + r * a.dim + i, a.dim - i);
             }
         }
     }
     if (!a.partial) return;
-    float* dst = a.partial + static_cast<int64_t>(blockIdx.x) * a.dim;
+    float* dst = a.partial + static_cast<int64_t>(blockIdx.x) * rms_partial_pitch(a.dim);
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
         const int i = (k * kGroup + t) * VEC;
@@ -329,7 +311,14 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 
 // copies), so what is in flight does not depend on registers; a row's stage is loaded again after the next row's
 // sum, when every thread has left it.  bf16, us (TB/s; loads into registers): 16384 x 8192 171 (6.3; 197), 32768 x 4096
 // 166 (6.5; 198), 65536 x 1024 101 (5.3; 119): a row of 1024 leaves little work between its two barriers.
-template <typename T, int kThreads, int KV>
+// Bytes of a ring's row: where rows start anywhere, room for the granules that they share with their neighbours.
+template <typename T>
+__host__ __device__ constexpr uint32_t ring_slot(int dim, bool aligned) {
+    const uint32_t bytes = static_cast<uint32_t>(dim) * sizeof(T);
+    return aligned ? bytes : (bytes + 15) / 16 * 16 + 16;
+}
+
+template <typename T, bool kAligned, int kThreads, int KV>
 __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, int stages) {
     constexpr int VEC = VecOf<T>::kN;
     extern __shared__ __align__(128) unsigned char ring[];
@@ -337,7 +326,7 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
     __shared__ uint64_t full[kRingStages];
     __shared__ int abort;
     const int t = threadIdx.x;
-    const uint32_t row_bytes = static_cast<uint32_t>(a.dim) * sizeof(T);
+    const uint32_t row_bytes = static_cast<uint32_t>(a.dim) * sizeof(T), slot = ring_slot<T>(a.dim, kAligned);
     const int inputs = a.gh ? 3 : 2;
     const int64_t first = blockIdx.x, step = gridDim.x;
     const int count = first < a.rows ? static_cast<int>((a.rows - 1 - first) / step) + 1 : 0;
@@ -348,18 +337,29 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
+    auto start = [&](int i, int64_t r) {      // row r of h, gy or gh
+        const void* p = i == 0 ? a.h : (i == 1 ? a.gy : a.gh);
+        return reinterpret_cast<uintptr_t>(static_cast<const T*>(p) + r * (i == 0 ? a.ldh : (i == 1 ? a.ldgy : a.ldgh)));
+    };
     auto load = [&](int j) {     // (thread 0) row j of this CTA
         const int s = j % stages;
         const int64_t r = first + j * step;
-        const uint32_t dst = tc::smem_u32(ring) + s * 3 * row_bytes, bar = tc::smem_u32(&full[s]);
-        tc::mbar_expect_tx(&full[s], inputs * row_bytes);
-        const T* src[3] = {static_cast<const T*>(a.h) + r * a.ldh, static_cast<const T*>(a.gy) + r * a.ldgy,
-                           static_cast<const T*>(a.gh) + r * a.ldgh};
-        for (int i = 0; i < inputs; ++i)
-            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                             dst + i * row_bytes),
-                         "l"(src[i]), "r"(row_bytes), "r"(bar)
-                         : "memory");
+        const uint32_t dst = tc::smem_u32(ring) + s * 3 * slot, bar = tc::smem_u32(&full[s]);
+        const uintptr_t src[3] = {start(0, r), start(1, r), start(2, r)};
+        uint32_t bytes[3], all = 0;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {      // whole 16-byte granules
+            bytes[i] = kAligned ? row_bytes : (static_cast<uint32_t>(src[i] & 15) + row_bytes + 15) & ~15u;
+            if (i < inputs) all += bytes[i];
+        }
+        tc::mbar_expect_tx(&full[s], all);
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (i < inputs)
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                 dst + i * slot),
+                             "l"(src[i] & ~uintptr_t(15)), "r"(bytes[i]), "r"(bar)
+                             : "memory");
     };
     if (t == 0)
         for (int j = 0; j < min(count, stages - 1); ++j) load(j);
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
         const int i = (k * kThreads + t) * VEC;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[k][e] = w[k][e] = 0.f;
-        if (i < a.dim) load_w<T, VEC>(a.w, a.w_f32, i, w[k]);
+        if (i < a.dim) load_w<T, kAligned>(a.w, a.w_f32, i, a.dim - i, w[k]);
     }
     const float inv_dim = 1.f / static_cast<float>(a.dim);
     for (int j = 0; j < count; ++j) {
@@ -377,15 +377,21 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
         const int64_t r = first + j * step;
         const float rstd = a.rstd[r];
         const bool here = tc::mbar_wait(&full[s], (j / stages) & 1, &abort);
-        const T* row = reinterpret_cast<const T*>(ring + s * 3 * row_bytes);
+        const T* in[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            in[i] = reinterpret_cast<const T*>(ring + (s * 3 + i) * slot + (kAligned ? 0 : start(i, r) & 15));
         float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
             const int i = (k * kThreads + t) * VEC;
             if (i < a.dim) {
                 float h[VEC], g[VEC];
-                load_vec<T, VEC>(row + i, h);
-                load_vec<T, VEC>(row + a.dim + i, g);
+                Raw<T, kAligned> v;
+                v.load(in[0] + i, a.dim - i);
+                v.get(h);
+                v.load(in[1] + i, a.dim - i);
+                v.get(g);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     acc[k][e] = fmaf(g[e], h[e] * rstd, acc[k][e]);
@@ -406,21 +412,26 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
             const int i = (k * kThreads + t) * VEC;
             if (i < a.dim) {
                 float h[VEC], g[VEC];
-                load_vec<T, VEC>(row + i, h);
-                load_vec<T, VEC>(row + a.dim + i, g);
+                Raw<T, kAligned> v;
+                v.load(in[0] + i, a.dim - i);
+                v.get(h);
+                v.load(in[1] + i, a.dim - i);
+                v.get(g);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) g[e] = fmaf(rstd, g[e] * w[k][e], -c * h[e]);
                 if (a.gh) {
-                    load_vec<T, VEC>(row + 2 * a.dim + i, h);
+                    v.load(in[2] + i, a.dim - i);
+                    v.get(h);
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) g[e] += h[e];
                 }
-                store_vec<T, VEC>(static_cast<T*>(a.gx) + r * a.dim + i, g);
+                v.set(g);
+                v.store(static_cast<T*>(a.gx) + r * a.dim + i, a.dim - i);
             }
         }
     }
     if (!a.partial) return;
-    float* dst = a.partial + static_cast<int64_t>(blockIdx.x) * a.dim;
+    float* dst = a.partial + static_cast<int64_t>(blockIdx.x) * rms_partial_pitch(a.dim);
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
         const int i = (k * kThreads + t) * VEC;
@@ -441,7 +452,7 @@ __global__ void __launch_bounds__(256) rms_gw_kernel(const float* __restrict__ p
     float s = 0.f;
     if (c < dim) {
 #pragma unroll 8
-        for (int r = y; r < rows; r += 8) s += partial[static_cast<int64_t>(r) * dim + c];
+        for (int r = y; r < rows; r += 8) s += partial[static_cast<int64_t>(r) * rms_partial_pitch(dim) + c];
     }
     red[y][threadIdx.x & 31] = s;
     __syncthreads();
@@ -454,46 +465,20 @@ __global__ void __launch_bounds__(256) rms_gw_kernel(const float* __restrict__ p
     }
 }
 
-// Threads per row and vectors per thread: the smallest group that holds `elems` (a warp while a thread
-// keeps at most 4 vectors, i.e. 1024 16-bit elements).
-template <int VEC, typename Fn>
-cudaError_t by_width(int elems, Fn&& fn) {
-    auto go = [&](auto g, auto kv) { return fn(g, kv); };
+// Threads per row and vectors per thread for rows of `vecs` 16-byte vectors: the smallest group that holds them, a
+// warp while a thread keeps at most 4.
+template <bool kLong, typename Fn>
+cudaError_t by_width(int vecs, Fn&& fn) {
 #define MMLTK_RMS_WIDTH(G, KV) \
-    if (elems <= G * KV * VEC) return go(std::integral_constant<int, G>{}, std::integral_constant<int, KV>{})
-    if constexpr (VEC == 1) {
-        MMLTK_RMS_WIDTH(128, 8);
-        MMLTK_RMS_WIDTH(256, 16);
-        MMLTK_RMS_WIDTH(512, 32);
-    } else {
-        MMLTK_RMS_WIDTH(32, 1);
-        MMLTK_RMS_WIDTH(32, 2);
-        MMLTK_RMS_WIDTH(32, 4);
-        MMLTK_RMS_WIDTH(128, 2);
-        MMLTK_RMS_WIDTH(128, 4);
-        MMLTK_RMS_WIDTH(256, 4);
-        MMLTK_RMS_WIDTH(512, 4);
-        if constexpr (VEC == 4) MMLTK_RMS_WIDTH(512, 8);
-    }
-#undef MMLTK_RMS_WIDTH
-    return cudaErrorInvalidValue;
-}
-
-// Rows that the ring does not take: of up to two vectors a thread of a warp, unaligned ones, and long fp32 ones.
-template <typename T, int VEC, typename Fn>
-cudaError_t by_width_bwd(int elems, Fn&& fn) {
-    auto go = [&](auto g, auto kv) { return fn(g, kv); };
-#define MMLTK_RMS_WIDTH(G, KV) \
-    if (elems <= G * KV * VEC) return go(std::integral_constant<int, G>{}, std::integral_constant<int, KV>{})
-    if constexpr (VEC == 1) {
-        MMLTK_RMS_WIDTH(128, 8);
-        MMLTK_RMS_WIDTH(512, 8);
-        MMLTK_RMS_WIDTH(1024, 16);
-    } else {
-        MMLTK_RMS_WIDTH(32, 1);
-        MMLTK_RMS_WIDTH(32, 2);
-        if constexpr (sizeof(T) == 4) MMLTK_RMS_WIDTH(1024, 4);
-    }
+    if (vecs <= G * KV) return fn(std::integral_constant<int, G>{}, std::integral_constant<int, KV>{})
+    MMLTK_RMS_WIDTH(32, 1);
+    MMLTK_RMS_WIDTH(32, 2);
+    MMLTK_RMS_WIDTH(32, 4);
+    MMLTK_RMS_WIDTH(128, 2);
+    MMLTK_RMS_WIDTH(128, 4);
+    MMLTK_RMS_WIDTH(256, 4);
+    MMLTK_RMS_WIDTH(512, 4);
+    if constexpr (kLong) MMLTK_RMS_WIDTH(512, 8);      // fp32
 #undef MMLTK_RMS_WIDTH
     return cudaErrorInvalidValue;
 }
@@ -511,37 +496,29 @@ cudaError_t launch_rms_fwd(Elt et, const RmsFwdArgs& a, cudaStream_t st) {
     return MMLTK_DISPATCH_ELT(et, [&]() -> cudaError_t {
         using T = elt_t;
         constexpr int kN = VecOf<T>::kN;
-        const bool vec = a.dim % kN == 0 && a.ldx % kN == 0 && aligned(a.x) && aligned(a.w) &&
-                         (!a.res || (a.ldr % kN == 0 && aligned(a.res)));
-        auto run = [&](auto vc) -> cudaError_t {
-            constexpr int VEC = decltype(vc)::value;
-            return by_width<VEC>(elems, [&](auto gc, auto kc) -> cudaError_t {
+        if (!aligned(a.w)) return cudaErrorInvalidValue;
+        const bool whole = a.dim % kN == 0 && a.ldx % kN == 0 && aligned(a.x) &&
+                           (!a.res || (a.ldr % kN == 0 && aligned(a.res)));
+        auto run = [&](auto ac) -> cudaError_t {
+            constexpr bool kAligned = decltype(ac)::value;
+            return by_width<sizeof(T) == 4>((elems + kN - 1) / kN, [&](auto gc, auto kc) -> cudaError_t {
                 constexpr int G = decltype(gc)::value, KV = decltype(kc)::value;
                 const int64_t per = G == 32 ? 8 : 1, blocks = (rows + per - 1) / per;
                 if (blocks >= (int64_t(1) << 31)) return cudaErrorInvalidValue;
                 const int threads = G == 32 ? 256 : G;
                 if (quant)
-                    rms_fwd_kernel<T, VEC, G, KV, true><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
+                    rms_fwd_kernel<T, kAligned, G, KV, true><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
                 else
-                    rms_fwd_kernel<T, VEC, G, KV, false><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
+                    rms_fwd_kernel<T, kAligned, G, KV, false><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
                 return cudaGetLastError();
             });
         };
-        if (vec) return run(std::integral_constant<int, kN>{});
-        return run(std::integral_constant<int, 1>{});
+        return whole ? run(std::true_type{}) : run(std::false_type{});
     });
 }
 
 namespace {
-// CTAs of the backward: 1024 threads an SM, fewer for few rows
-int bwd_blocks(int64_t rows, int group) {
-    const int64_t per = group == 32 ? 8 : 1;
-    const int per_sm = group == 32 ? 3 : (group >= 512 ? 1024 / group : 768 / group);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, num_sms() * per_sm)));
-}
-}  // namespace
 
-namespace {
 template <typename T>
 cudaError_t sum_gw(const RmsBwdArgs& a, int blocks, cudaStream_t st) {
     if (!a.partial) return cudaSuccess;
@@ -549,62 +526,65 @@ cudaError_t sum_gw(const RmsBwdArgs& a, int blocks, cudaStream_t st) {
     return cudaGetLastError();
 }
 
-// Rows of more than a warp's registers, 16-byte aligned.  As many CTAs an SM as keep three stages (two from 24 KB a
-// stage on): the barriers of one row are then under other rows' loads (16384 x 8192: 171 us with two CTAs of two
-// stages, 189 with one of four; 65536 x 1024: 101 with eight CTAs, 123 with four).
-template <typename T>
+// Rows of more than two vectors a lane.  As many CTAs an SM as keep three stages (two from 24 KB a stage on): the
+// barriers of one row are then under other rows' loads (16384 x 8192: 171 us with two CTAs of two stages, 189 with one
+// of four; 65536 x 1024: 101 with eight CTAs, 123 with four).  Not for fp32 rows of over 9000 elements, whose two
+// stages would not fit.
+template <typename T, bool kAligned>
 cudaError_t ring_bwd(const RmsBwdArgs& a, cudaStream_t st) {
-    const int vecs = a.dim / VecOf<T>::kN;
-    if (vecs <= 64) return cudaErrorNotSupported;
-    const int stage = 3 * a.dim * static_cast<int>(sizeof(T));
+    const int vecs = (a.dim + VecOf<T>::kN - 1) / VecOf<T>::kN;
+    const int stage = 3 * static_cast<int>(ring_slot<T>(a.dim, kAligned));
     const int per_sm = vecs <= 128 ? 8 : (vecs <= 256 ? 6 : (3 * stage <= 72 * 1024 ? 3 : (2 * stage <= 108 * 1024 ? 2 : 1)));
     const int stages = std::min(kRingStages, 216 * 1024 / per_sm / stage);
-    if (stages < 2) return cudaErrorNotSupported;
+    if (vecs <= 64 || vecs > 2048 || stages < 2) return cudaErrorNotSupported;
     const int blocks = static_cast<int>(std::min<int64_t>(a.rows, static_cast<int64_t>(num_sms()) * per_sm));
     auto run = [&](auto kern, int threads) -> cudaError_t {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, stages * stage);
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, stages * stage);
         if (e != cudaSuccess) return e;
         kern<<<blocks, threads, stages * stage, st>>>(a, stages);
-        e = cudaGetLastError();
-        return e != cudaSuccess ? e : sum_gw<T>(a, blocks, st);
+        const cudaError_t l = cudaGetLastError();
+        return l != cudaSuccess ? l : sum_gw<T>(a, blocks, st);
     };
-    if (vecs <= 128) return run(rms_bwd_ring_kernel<T, 128, 1>, 128);
-    if (vecs <= 256) return run(rms_bwd_ring_kernel<T, 128, 2>, 128);
-    if (vecs <= 512) return run(rms_bwd_ring_kernel<T, 256, 2>, 256);
-    if (vecs <= 1024) return run(rms_bwd_ring_kernel<T, 256, 4>, 256);
-    if (vecs <= 2048) return run(rms_bwd_ring_kernel<T, 512, 4>, 512);
-    return cudaErrorNotSupported;      // fp32 rows of over 8192 elements: two stages would not fit
+    if (vecs <= 128) return run(rms_bwd_ring_kernel<T, kAligned, 128, 1>, 128);
+    if (vecs <= 256) return run(rms_bwd_ring_kernel<T, kAligned, 128, 2>, 128);
+    if (vecs <= 512) return run(rms_bwd_ring_kernel<T, kAligned, 256, 2>, 256);
+    if (vecs <= 1024) return run(rms_bwd_ring_kernel<T, kAligned, 256, 4>, 256);
+    return run(rms_bwd_ring_kernel<T, kAligned, 512, 4>, 512);
 }
+
+template <typename T, bool kAligned>
+cudaError_t bwd(const RmsBwdArgs& a, cudaStream_t st) {
+    if (a.rows <= 0) return a.partial ? cudaMemsetAsync(a.gw, 0, a.dim * (a.w_f32 ? sizeof(float) : sizeof(T)), st) : cudaSuccess;
+    const cudaError_t e = ring_bwd<T, kAligned>(a, st);
+    if (e != cudaErrorNotSupported) return e;
+    const int vecs = (a.dim + VecOf<T>::kN - 1) / VecOf<T>::kN;
+    auto run = [&](auto kern, int rows_cta, int threads, int per_sm) -> cudaError_t {
+        const int blocks = static_cast<int>(std::max<int64_t>(
+            1, std::min<int64_t>((a.rows + rows_cta - 1) / rows_cta, static_cast<int64_t>(num_sms()) * per_sm)));
+        kern<<<blocks, threads, 0, st>>>(a);
+        const cudaError_t l = cudaGetLastError();
+        return l != cudaSuccess ? l : sum_gw<T>(a, blocks, st);
+    };
+    if (vecs <= 32) return run(rms_bwd_kernel<T, kAligned, 32, 1>, 8, 256, 3);
+    if (vecs <= 64) return run(rms_bwd_kernel<T, kAligned, 32, 2>, 8, 256, 3);
+    if constexpr (sizeof(T) == 4) return run(rms_bwd_kernel<T, kAligned, 1024, 4>, 1, 1024, 1);
+    return cudaErrorInvalidValue;
+}
+
 }  // namespace
 
-int rms_bwd_partials(Elt, int64_t rows, int) {
+int rms_bwd_partials(int64_t rows) {
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, num_sms() * 8)));
 }
 
 cudaError_t launch_rms_bwd(Elt et, const RmsBwdArgs& a, cudaStream_t st) {
-    if (a.dim <= 0 || a.dim > kRmsMaxDim) return cudaErrorInvalidValue;
+    if (a.dim <= 0 || a.dim > kRmsMaxDim || !aligned(a.w)) return cudaErrorInvalidValue;
     return MMLTK_DISPATCH_ELT(et, [&]() -> cudaError_t {
         using T = elt_t;
         constexpr int kN = VecOf<T>::kN;
-        const bool vec = a.dim % kN == 0 && aligned(a.h) && a.ldh % kN == 0 && aligned(a.w) &&
-                         a.ldgy % kN == 0 && aligned(a.gy) &&
-                         (!a.gh || (a.ldgh % kN == 0 && aligned(a.gh)));
-        if (vec && a.rows > 0) {
-            const cudaError_t e = ring_bwd<T>(a, st);
-            if (e != cudaErrorNotSupported) return e;
-        }
-        auto run = [&](auto vc) -> cudaError_t {
-            constexpr int VEC = decltype(vc)::value;
-            return by_width_bwd<T, VEC>(a.dim, [&](auto gc, auto kc) -> cudaError_t {
-                constexpr int G = decltype(gc)::value, KV = decltype(kc)::value;
-                const int blocks = bwd_blocks(a.rows, G);
-                rms_bwd_kernel<T, VEC, G, KV><<<blocks, G == 32 ? 256 : G, 0, st>>>(a);
-                const cudaError_t e = cudaGetLastError();
-                return e != cudaSuccess ? e : sum_gw<T>(a, blocks, st);
-            });
-        };
-        if (vec) return run(std::integral_constant<int, kN>{});
-        return run(std::integral_constant<int, 1>{});
+        const bool whole = a.dim % kN == 0 && aligned(a.h) && a.ldh % kN == 0 && a.ldgy % kN == 0 && aligned(a.gy) &&
+                           (!a.gh || (a.ldgh % kN == 0 && aligned(a.gh)));
+        return whole ? bwd<T, true>(a, st) : bwd<T, false>(a, st);
     });
 }
 
