@@ -128,21 +128,46 @@ __global__ void __launch_bounds__(512) mx_amax_kernel(const T* __restrict__ x, i
     if ((threadIdx.x & 31) == 0 && m) atomicMax(amax, m);
 }
 
+// 16 values of a lane to an unaligned place: the aligned granules between its vectors whole, the ends in pieces.
+template <typename T>
+__device__ __forceinline__ void lane_store(T* o, const float* v, int n) {
+    constexpr int kN = VecOf<T>::kN;
+    if (n < 16) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (e < n) o[e] = from_f<T>(v[e]);
+        return;
+    }
+    char* c = reinterpret_cast<char*>(o);
+    const uint32_t head = (16 - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(o) & 15)) & 15;
+    uint4 w = pack16(v, T());
+    if (head) store_part(c, w, 0, head);
+#pragma unroll
+    for (int e = kN; e < 16; e += kN) {
+        const uint4 u = pack16(v + e, T());
+        *reinterpret_cast<uint4*>(c + (e / kN - 1) * 16 + head) = head ? shift16(w, u, head) : w;
+        w = u;
+    }
+    c += (16 / kN - 1) * 16;
+    if (head) store_part(c, w, head, 16);
+    else *reinterpret_cast<uint4*>(c) = w;
+}
+
 // A thread writes 16 consecutive values (one 32-byte store of a 16-bit type); a CTA's y is a row of
 // CTAs, its x the columns.
-template <typename T, MxFormat F>
+template <typename T, MxFormat F, bool kWhole>     // kWhole: rows are 32-byte aligned
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __restrict__ codes, int64_t pitch,
                                                             const uint8_t* __restrict__ scales, int kt,
                                                             const float* __restrict__ g_in, int64_t rows, int64_t dim,
-                                                            int parts, int part_bits, T* __restrict__ out, int align) {
+                                                            int parts, int part_bits, T* __restrict__ out) {
     using Tr = Traits<F>;
     const float g = (!Tr::kPow2 && g_in) ? *g_in : 1.f;
     // 2^part_bits threads side by side in a row
     const int part0 = threadIdx.x & ((1 << part_bits) - 1), line = threadIdx.x >> part_bits, lines = 256 >> part_bits;
+    const int part = (blockIdx.x << part_bits) + part0;
     for (int64_t r = static_cast<int64_t>(blockIdx.y) * lines + line; r < rows; r += static_cast<int64_t>(gridDim.y) * lines) {
-        const int part = (blockIdx.x << part_bits) + part0;
-        if (part >= parts) return;
         const int64_t col = static_cast<int64_t>(part) * 16;
+        if (part >= parts) continue;
         const float s = scale_value<F>(scales[scale_offset(r, static_cast<int>(col / Tr::kBlock), kt)]);
         float v[16];
         if constexpr (Tr::kBits == 4) {
@@ -168,16 +193,11 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __res
         for (int e = 0; e < 16; ++e) v[e] = v[e] * s * g;
         T* o = out + r * dim + col;
         constexpr int kN = VecOf<T>::kN;
-        if (align == 2 && col + 16 <= dim) {
+        if (kWhole && col + 16 <= dim) {
 #pragma unroll
             for (int e = 0; e < 16; e += 2 * kN) st_global_32(o + e, pack16(v + e, T()), pack16(v + e + kN, T()));
-        } else if (align && col + 16 <= dim) {
-#pragma unroll
-            for (int e = 0; e < 16; e += kN) *reinterpret_cast<uint4*>(o + e) = pack16(v + e, T());
         } else {
-            const int n = static_cast<int>(dim - col < 16 ? dim - col : 16);
-#pragma unroll
-            for (int e = 0; e < 16; e += kN) store_any_vec(o + e, pack16(v + e, T()), n - e);
+            lane_store<T>(o, v, static_cast<int>(dim - col < 16 ? dim - col : 16));
         }
     }
 }
@@ -253,11 +273,14 @@ cudaError_t launch_mx_dequantize(Elt et, MxFormat f, const void* codes, const vo
         const int align = row_align(out, dim * static_cast<int64_t>(sizeof(T)));
         return by_format(f, [&](auto fc) -> cudaError_t {
             constexpr MxFormat F = decltype(fc)::value;
-            mx_dequantize_kernel<T, F><<<grid, 256, 0, st>>>(
-                static_cast<const uint8_t*>(codes), mx_pitch(f, dim), static_cast<const uint8_t*>(scales),
-                static_cast<int>(mx_scale_tiles(f, dim)), g, rows, dim, static_cast<int>(parts), bits,
-                static_cast<T*>(out), align);
-            return cudaGetLastError();
+            auto run = [&](auto kern) {
+                kern<<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(codes), mx_pitch(f, dim),
+                                           static_cast<const uint8_t*>(scales), static_cast<int>(mx_scale_tiles(f, dim)),
+                                           g, rows, dim, static_cast<int>(parts), bits, static_cast<T*>(out));
+                return cudaGetLastError();
+            };
+            if (align == 2) return run(mx_dequantize_kernel<T, F, true>);
+            return run(mx_dequantize_kernel<T, F, false>);
         });
     });
 }

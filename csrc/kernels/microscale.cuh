@@ -266,6 +266,24 @@ __device__ __forceinline__ uint4 load_any(const T* p, int n) {
     }
     return w;
 }
+// Bytes from .. to - 1 of w (multiples of the element size) at p + from, where p + from or p + to is 16-byte aligned:
+// pieces of 2, 4 and 8 bytes, rising from an unaligned start or falling from an aligned one.
+__device__ __forceinline__ void store_part(char* p, const uint4& w, uint32_t from, uint32_t to) {
+    const bool rising = (reinterpret_cast<uintptr_t>(p + from) & 15) != 0;
+    const uint32_t count = to - from;
+    uint32_t at = from;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        const uint32_t size = rising ? 2u << k : 8u >> k;
+        if (count & size) {
+            const uint4 v = shift16(w, make_uint4(0, 0, 0, 0), at);
+            if (size == 2) *reinterpret_cast<unsigned short*>(p + at) = static_cast<unsigned short>(v.x);
+            else if (size == 4) *reinterpret_cast<uint32_t*>(p + at) = v.x;
+            else *reinterpret_cast<uint2*>(p + at) = make_uint2(v.x, v.y);
+            at += size;
+        }
+    }
+}
 // Stores the first n elements of w at p, in the widest pieces that p's address allows.
 template <typename T>
 __device__ __forceinline__ void store_any_vec(T* p, const uint4& w, int n) {

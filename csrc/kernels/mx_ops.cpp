@@ -1,5 +1,7 @@
 // Torch wrappers of the microscaled formats, their products and the RMS norm.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <limits>
@@ -31,6 +33,17 @@ MxFormat format_of(int64_t f) {
     return static_cast<MxFormat>(f);
 }
 
+// A new tensor without a trip through the dispatcher (half of torch::empty's 1.7 us, and a small call makes three).
+torch::Tensor fresh(at::IntArrayRef sizes, torch::ScalarType dtype, const torch::Tensor& like) {
+    return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
+}
+// Work space of the current stream, given back to the allocator at the end of the scope.
+struct WorkSpace {
+    explicit WorkSpace(int64_t bytes) : block(c10::cuda::CUDACachingAllocator::get()->allocate(static_cast<size_t>(bytes))) {}
+    void* at(int64_t offset) const { return static_cast<char*>(block.get()) + offset; }
+    c10::DataPtr block;
+};
+
 bool aligned16(const torch::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
 // x [..., K] as rows of K elements, a view where its strides allow one
@@ -56,10 +69,10 @@ torch::ScalarType code_type(MxFormat f) {
     return f == MxFormat::kMxFp8 ? torch::ScalarType::Float8_e4m3fn : torch::kUInt8;
 }
 torch::Tensor new_codes(MxFormat f, int64_t rows, int64_t dim, const torch::Tensor& like) {
-    return torch::empty({rows, mx_pitch(f, dim)}, like.options().dtype(code_type(f)));
+    return fresh({rows, mx_pitch(f, dim)}, code_type(f), like);
 }
 torch::Tensor new_scales(MxFormat f, int64_t rows, int64_t dim, const torch::Tensor& like) {
-    return torch::empty({(rows + 127) / 128, mx_scale_tiles(f, dim), 32, 4, 4}, like.options().dtype(torch::kUInt8));
+    return fresh({(rows + 127) / 128, mx_scale_tiles(f, dim), 32, 4, 4}, torch::kUInt8, like);
 }
 void check_coded(MxFormat f, const torch::Tensor& codes, const torch::Tensor& scales, int64_t rows, int64_t dim,
                  const char* what) {
@@ -113,22 +126,23 @@ std::vector<OptTensor> mx_quantize(torch::Tensor x, int64_t fmt, OptTensor g) {
     const torch::Tensor r = as_rows(x);
     const int64_t rows = r.size(0), dim = r.size(1);
     auto codes = new_codes(f, rows, dim, x), scales = new_scales(f, rows, dim, x);
-    torch::Tensor gt, work;
+    torch::Tensor gt;
+    c10::optional<WorkSpace> work;
     if (f == MxFormat::kNvFp4) {
         if (has(g)) {
             check_scalar(*g, x, "mx_quantize");
             gt = *g;
         } else {
-            gt = rows ? torch::empty({1}, x.options().dtype(torch::kFloat32))
+            gt = rows ? fresh({1}, torch::kFloat32, x)
                       : torch::ones({1}, x.options().dtype(torch::kFloat32));
-            work = torch::empty({1}, x.options().dtype(torch::kInt32));
+            work.emplace(sizeof(uint32_t));
         }
     } else {
         TORCH_CHECK(!has(g), "mx_quantize: only nvfp4 has a tensor scale");
     }
     check_cuda(launch_mx_quantize(et, f, r.data_ptr(), row_pitch(r), rows, dim, codes.data_ptr(), scales.data_ptr(),
                                   gt.defined() ? gt.data_ptr<float>() : nullptr,
-                                  work.defined() ? reinterpret_cast<uint32_t*>(work.data_ptr<int>()) : nullptr,
+                                  work ? static_cast<uint32_t*>(work->at(0)) : nullptr,
                                   cur_stream()),
                "mx_quantize");
     return {codes, scales, gt.defined() ? OptTensor(gt) : OptTensor()};
@@ -140,7 +154,7 @@ torch::Tensor mx_dequantize(torch::Tensor codes, torch::Tensor scales, OptTensor
     check_coded(f, codes, scales, rows, dim, "mx_dequantize");
     if (has(g)) check_scalar(*g, codes, "mx_dequantize");
     at::cuda::CUDAGuard guard(codes.device());
-    auto out = torch::empty({rows, dim}, codes.options().dtype(dtype));
+    auto out = fresh({rows, dim}, dtype, codes);
     check_cuda(launch_mx_dequantize(elt_of(out, "mx_dequantize"), f, codes.data_ptr(), scales.data_ptr(),
                                     has(g) ? g->data_ptr<float>() : nullptr, rows, dim, out.data_ptr(), cur_stream()),
                "mx_dequantize");
@@ -182,14 +196,14 @@ NormOut norm_forward(const torch::Tensor& x, const torch::Tensor& w_in, const Op
         rr = as_rows(*res);
         a.res = rr.data_ptr();
         a.ldr = row_pitch(rr);
-        o.h = torch::empty(x.sizes(), x.options());
+        o.h = fresh(x.sizes(), x.scalar_type(), x);
         a.h = o.h.data_ptr();
     }
     a.w = w.data_ptr();
     a.w_f32 = w.scalar_type() == torch::kFloat32 && x.scalar_type() != torch::kFloat32;
     a.eps = static_cast<float>(eps);
     if (want_rstd) {
-        o.rstd = torch::empty({a.rows}, x.options().dtype(torch::kFloat32));
+        o.rstd = fresh({a.rows}, torch::kFloat32, x);
         a.rstd = o.rstd.data_ptr<float>();
     }
     if (fmt) {
@@ -200,7 +214,7 @@ NormOut norm_forward(const torch::Tensor& x, const torch::Tensor& w_in, const Op
         a.g = g;
         a.fmt = *fmt;
     } else {
-        o.y = torch::empty(x.sizes(), x.options());
+        o.y = fresh(x.sizes(), x.scalar_type(), x);
         a.y = o.y.data_ptr();
     }
     if (a.rows) check_cuda(launch_rms_fwd(elt_of(x, what), a, cur_stream()), what);
@@ -231,15 +245,16 @@ std::pair<torch::Tensor, torch::Tensor> norm_backward(const torch::Tensor& gy, c
     a.w_f32 = w.scalar_type() == torch::kFloat32 && h.scalar_type() != torch::kFloat32;
     a.rstd = rstd.data_ptr<float>();
     a.status = mx_status_word(h.device());
-    auto gx = torch::empty(h.sizes(), h.options());
+    auto gx = fresh(h.sizes(), h.scalar_type(), h);
     a.gx = gx.data_ptr();
-    torch::Tensor gw, partial;
+    torch::Tensor gw;
+    c10::optional<WorkSpace> partial;
     const Elt et = elt_of(h, "rms_norm backward");
     if (want_gw) {
-        gw = torch::empty(w.sizes(), w.options());
+        gw = fresh(w.sizes(), w.scalar_type(), w);
         a.gw = gw.data_ptr();
-        partial = torch::empty({rms_bwd_partials(a.rows), rms_partial_pitch(a.dim)}, h.options().dtype(torch::kFloat32));
-        a.partial = partial.data_ptr<float>();
+        partial.emplace(static_cast<int64_t>(rms_bwd_partials(a.rows)) * rms_partial_pitch(a.dim) * sizeof(float));
+        a.partial = static_cast<float*>(partial->at(0));
     }
     check_cuda(launch_rms_bwd(et, a, cur_stream()), "rms_norm backward");
     return {gx, gw};
@@ -353,7 +368,7 @@ std::vector<torch::Tensor> mx_linear(OptTensor x, OptTensor x_codes, OptTensor x
         a.scales = scales.data_ptr();
         a.y_pitch = mx_pitch(MxFormat::kMxFp8, n);
     } else {
-        y = torch::empty({rows, n}, w_codes.options().dtype(out_dtype));
+        y = fresh({rows, n}, out_dtype, w_codes);
         a.out = elt_of(y, "mx_linear: output");
         a.y = y.data_ptr();
         a.y_pitch = n * static_cast<int64_t>(y.element_size());
@@ -375,15 +390,19 @@ std::vector<torch::Tensor> mx_linear(OptTensor x, OptTensor x_codes, OptTensor x
             if (quant_out) return {codes, scales};
             return {y};
         }
+        c10::optional<WorkSpace> xq;
         if (xr.defined()) {
-            xc = new_codes(f, rows, k, w_codes);
-            xs = new_scales(f, rows, k, w_codes);
-            check_cuda(launch_mx_quantize(elt_of(xr, "mx_linear"), f, xr.data_ptr(), row_pitch(xr), rows, k,
-                                          xc.data_ptr(), xs.data_ptr(), const_cast<float*>(a.x_g), nullptr, cur_stream()),
+            const int64_t code_bytes = (rows * a.x_pitch + 511) / 512 * 512;
+            xq.emplace(code_bytes + (rows + 127) / 128 * mx_scale_tiles(f, k) * 512);
+            check_cuda(launch_mx_quantize(elt_of(xr, "mx_linear"), f, xr.data_ptr(), row_pitch(xr), rows, k, xq->at(0),
+                                          xq->at(code_bytes), const_cast<float*>(a.x_g), nullptr, cur_stream()),
                        "mx_linear: quantisation");
+            a.x_codes = xq->at(0);
+            a.x_scales = xq->at(code_bytes);
+        } else {
+            a.x_codes = xc.data_ptr();
+            a.x_scales = xs.data_ptr();
         }
-        a.x_codes = xc.data_ptr();
-        a.x_scales = xs.data_ptr();
         check_cuda(launch_mx_gemm(a, cur_stream()), "mx_linear");
     }
     if (quant_out) return {codes, scales};
