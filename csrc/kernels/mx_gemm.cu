@@ -27,6 +27,13 @@
 // registers took as long as the rest of a short product together).  The quantised output (mxfp8) needs
 // no second pass: a thread has 32 consecutive columns of a row, one scale block.
 //
+// Measured (B200, CUDA-graph replays): 8192^3 mxfp8 375 us (2.9 PFLOP/s), mxfp4 197 us (5.6), nvfp4 222 us (5.0).  These
+// run at the power cap (1.35 to 1.55 GHz; a bf16 cuBLAS product there 1.1 PFLOP/s); the tensor pipe is busy
+// 74 % of the cycles (4096^3 mxfp8).  nvfp4 is slower than mxfp4 by its scale copies: 12 a stage take 132
+// cycles beside the MMAs' 512, 6 take 52, 3 none.  Short products are bound by issue slots: at
+// 31200 x 2048 x 256 to mxfp8 (30 us; 66 MB out, 10 us) the epilogue's warps use 58 % of them, and the
+// scheduler keeps a ready warp going, so the issuing warp waits for the epilogue's bursts.
+//
 // Every wait is bounded: on a time-out the kernel records which role gave up in a status word and
 // leaves, after releasing its tensor memory.
 #include "mx_mma.cuh"
@@ -660,11 +667,11 @@ cudaError_t by_output(const MxGemmArgs& g, cudaStream_t st) {
 
 template <MxFormat F>
 cudaError_t by_tile(const MxGemmArgs& g, cudaStream_t st) {
-    // Pairs where the reduction is long (8 stages) and the pairs get two tiles each: at 8192^3 they take 388 us where
-    // 128 x 256 tiles of single CTAs take 462 (mxfp8) and 222 against 314 (nvfp4); at K = 256 they lose (31200 x 2048:
-    // 46 us against 32), each tile's hand-overs crossing the pair.  Else the width whose waves cost less, a
-    // 256-column tile counting 1.75 of a 128-column one (31200 x 2048 x 256: 33.5 and 31; 10400 x 1536 x 384: 19.0
-    // and 19.8; 512 x 4096 x 4096: 10.7 and 14.1).
+    // Pairs where the reduction is long (8 stages) and the pairs get two tiles each: at 8192^3 they take 392 us where
+    // 128 x 256 tiles of single CTAs take 462 (mxfp8) and 224 against 318 (nvfp4); at K = 256 they lose (31200 x 2048:
+    // 45 us against 30), each tile's hand-overs crossing the pair.  Else the width whose waves cost less, a
+    // 256-column tile counting 1.75 of a 128-column one (31200 x 2048 x 256: 33.4 and 30.0; 10400 x 1536 x 384: 18.3
+    // and 19.6; 512 x 4096 x 4096: 9.9 and 13.6).
     const int64_t sms = num_sms(), rt = (g.m + 127) / 128;
     const int64_t pairs = (rt + 1) / 2 * ((g.n + 255) / 256);
     if (g.k >= 8 * Kind<F>::kElems && pairs >= sms) return by_output<F, 256, true>(g, st);
