@@ -132,24 +132,35 @@ __device__ __forceinline__ void staging_store(int lane, const CUtensorMap* map, 
     }
 }
 
-// Output rows that are no multiple of 16 bytes: 32 x 32 values (a row's in w) through shared memory, 32 bytes of a
-// row at a time, so that a warp writes row segments.
-template <typename O>
-__device__ __forceinline__ void store_any(const MxGemmArgs& g, unsigned char* buf, int lane, const uint32_t* w, int col,
-                                          int row0) {
-    constexpr int kCols = 32 / sizeof(O);
-#pragma unroll
-    for (int part = 0; part < 32 / kCols; ++part) {
-        const int c = col + part * kCols + lane % kCols;
-        uint4* rowp = reinterpret_cast<uint4*>(buf + lane * 32);
-        rowp[0] = make_uint4(w[8 * part], w[8 * part + 1], w[8 * part + 2], w[8 * part + 3]);
-        rowp[1] = make_uint4(w[8 * part + 4], w[8 * part + 5], w[8 * part + 6], w[8 * part + 7]);
-        __syncwarp();
-        for (int r = lane / kCols; r < 32 && row0 + r < g.m; r += 32 / kCols)
-            if (c < g.n)
-                static_cast<O*>(g.y)[static_cast<int64_t>(row0 + r) * g.n + c] =
-                    reinterpret_cast<const O*>(buf + r * 32)[lane % kCols];
-        __syncwarp();
+// Output rows that are no multiple of 16 bytes, from a staging tile at (row0, col0): a lane writes 4 bytes of a row (the
+// warp one row of 128 bytes or two of 64).  A 16-bit row that starts between two words is shifted by an element, its first
+// and last one written alone.
+template <typename O, int kRow>
+__device__ __forceinline__ void copy_rows(const MxGemmArgs& g, const unsigned char* buf, int lane, int col0, int row0) {
+    constexpr int kWords = kRow / 4, kPer = 32 / kWords;
+    const int rows = min(32, g.m - row0), cols = min(kRow / static_cast<int>(sizeof(O)), g.n - col0);
+    const int l = lane % kWords;
+    auto word = [&](int r, int j) {
+        const int sw = kRow == 128 ? r & 7 : (r >> 1) & 3;
+        return *reinterpret_cast<const uint32_t*>(buf + r * kRow + ((((j >> 2) ^ sw) << 4) | ((j & 3) << 2)));
+    };
+    __syncwarp();
+    O* p = static_cast<O*>(g.y) + static_cast<int64_t>(row0 + lane / kWords) * g.n + col0;
+    const int64_t step = static_cast<int64_t>(kPer) * g.n;
+#pragma unroll 4
+    for (int r = lane / kWords; r < rows; r += kPer, p += step) {
+        const uint32_t a = word(r, l);
+        if constexpr (sizeof(O) == 4) {
+            if (l < cols) reinterpret_cast<uint32_t*>(p)[l] = a;
+        } else {
+            const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1, e = 2 * l + odd;
+            const uint32_t b = word(r, min(l + 1, kWords - 1));
+            const uint32_t v = odd ? __funnelshift_r(a, b, 16) : a;
+            unsigned short* q = reinterpret_cast<unsigned short*>(p);
+            if (e + 1 < cols) *reinterpret_cast<uint32_t*>(q + e) = v;
+            else if (e < cols) q[e] = static_cast<unsigned short>(v);
+            if (odd && l == 0) q[0] = static_cast<unsigned short>(a);
+        }
     }
 }
 
@@ -480,6 +491,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                    : g.bias_elt == Elt::kBF16 ? to_f(static_cast<const __nv_bfloat16*>(g.bias)[col])
                                               : to_f(static_cast<const __half*>(g.bias)[col]);
         };
+        auto flush = [&](int col, int row0) {      // the staging tile's columns from col on
+            if constexpr (kQuantOut) {
+                staging_store(lane, &tmY, buf_s, col, row0);
+            } else {
+                if (tensor_store) staging_store(lane, &tmY, buf_s, col, row0);
+                else copy_rows<O, kRow>(g, buf_s, lane, col, row0);
+            }
+        };
         int mt = 0, nt = 0, mt_next = 0, nt_next = 0;
         float bias_r[kChunks];
         if (first < sch.units) {
@@ -559,10 +578,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int j = 0; j < 16; ++j) convert2<O, false>(x[j], w + j * kSize / 2);
                 }
-                if (!tensor_store) {
-                    if constexpr (!kQuantOut) store_any<O>(g, buf_s, lane, w, col, row0);
-                    continue;
-                }
                 if (freed == 0 || kBox == 32) {
                     staging_free(lane);
                     freed = 1;
@@ -571,9 +586,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = 0; j < kPieces; ++j)
                     *staged<kRow>(buf_s, lane, (kBox == 32 ? 0 : c * kPieces) + j) =
                         make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-                if (kBox == 32) staging_store(lane, &tmY, buf_s, col, row0);
+                if (kBox == 32) flush(col, row0);
             }
-            if (kBox > 32 && tensor_store && col0 < g.n && row0 < g.m) staging_store(lane, &tmY, buf_s, col0, row0);
+            if (kBox > 32 && col0 < g.n && row0 < g.m) flush(col0, row0);
             if constexpr (kQuantOut) {
                 // scale bytes of this row's blocks: one or two neighbours; zero past m and n
                 if (row0 / 128 < (g.m + 127) / 128 && col0 / 128 < ykt) {
