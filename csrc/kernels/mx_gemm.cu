@@ -92,6 +92,7 @@ struct __align__(8) Ctl {
 
 struct Sched {
     int m_tiles, n_tiles, ktiles, units;
+    int splits, kt_per;           // slices of the reduction (the CTAs of a cluster) and their stages
     uint32_t per, magic;          // tiles of a group of 8 row tiles, and 2^32 / per
     // groups of 8 row tiles, column by column inside a group: the tiles in flight share operand rows in L2.
     // (Every role walks the tiles; plain divisions here cost the loading warp a third of a short tile's time.)
@@ -301,7 +302,10 @@ __device__ __forceinline__ void tmem_settle(uint32_t* r) {
                  : "memory");
 }
 
-template <MxFormat F, int BN_, bool kPair, typename O, bool kQuantOut>
+// kSplit: few tiles and a long reduction.  Each CTA of a cluster multiplies a slice of it for the same 128 x 128 tile;
+// the partial sums meet in shared memory, and each CTA finishes its share of the column quarters, adding the slices
+// in their order.
+template <MxFormat F, int BN_, bool kPair, bool kSplit, typename O, bool kQuantOut>
 __global__ void __launch_bounds__(kThreads, 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
@@ -323,7 +327,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     // asynchronous instructions take their operands from
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = kPair ? blockIdx.x & 1 : 0;
-    const int first = kPair ? blockIdx.x >> 1 : blockIdx.x, step = kPair ? gridDim.x >> 1 : gridDim.x;
+    const int slice = kSplit ? blockIdx.x % sch.splits : 0;
+    const int first = kSplit ? blockIdx.x / sch.splits : (kPair ? blockIdx.x >> 1 : blockIdx.x);
+    const int step = kSplit ? sch.units : (kPair ? gridDim.x >> 1 : gridDim.x);      // (kSplit: one tile a cluster)
+    const int kt0 = kSplit ? slice * sch.kt_per : 0, kts = kSplit ? min(sch.kt_per, sch.ktiles - kt0) : sch.ktiles;
+    static_assert(!kSplit || (BN == 128 && !kPair));
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -368,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             int mt, nt;
             sch.tile(u, mt, nt);
             const int rt = kPair ? 2 * mt + rank : mt;      // this CTA's tile of 128 rows
-            for (int kt = 0; kt < sch.ktiles; ++kt) {
+            for (int kt = kt0; kt < kt0 + kts; ++kt) {
                 if (!__all_sync(0xffffffffu, mbar_wait(&ctl->empty[s], phase, &ctl->abort))) {
                     if (elected) {
                         ctl->abort = 1;
@@ -389,7 +397,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
-    producer_done:;
+    producer_done:
+        if constexpr (kSplit) cluster_sync_all();
     } else if (warp == 1) {
         if (rank == 0) {
             const uint32_t elected = elect_lane();
@@ -417,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 tc_fence_after();
                 const uint32_t acc = tmem + buf * C::kAcc1;
-                int left = g.k;
+                int left = kSplit ? min(g.k - kt0 * K::kElems, kts * K::kElems) : g.k;
                 uint32_t more = 0;
                 for (; ok && left > 0; left -= K::kElems) {
                     if (!ready) ok = __all_sync(0xffffffffu, mbar_wait(&ctl->full[s], phase, &ctl->abort));
@@ -476,6 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
+        if constexpr (kSplit) cluster_sync_all();
     } else {
         // sixteen warps (four a scheduler hide the latencies of a chunk): lane quarter q, column quarter part
         const int q = warp & 3, part = (warp - 2) >> 2;
@@ -525,6 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!mbar_wait(&ctl->acc_full[buf], (local >> 1) & 1, &ctl->abort)) {
                 if (lane == 0) atomicCAS(g.status, 0, 3);
                 ctl->abort = 1;
+                if constexpr (kSplit) cluster_sync_all();
                 break;
             }
             tc_fence_after();
@@ -533,6 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int mine = buf ? min(kChunks, C::kShared - part * kChunks)
                                  : min(kChunks, C::kShared - (3 - part) * kChunks);     // how many, if positive
             uint32_t bytes = 0, freed = 0;
+            bool owner = true;
 #pragma unroll
             for (int i = 0; i < kChunks; ++i) {
                 const int c = buf ? i : kChunks - 1 - i;
@@ -553,6 +565,40 @@ __global__ void __launch_bounds__(kThreads, 1)
                             else mbar_arrive(&ctl->acc_empty[buf]);
                         }
                     }
+                }
+                if constexpr (kSplit) {
+                    // every operand stage has been used: their room takes the partial sums
+                    const uint32_t at = smem_u32(tilesA) + (part * 4 + q) * 4096 + lane * 16;
+                    owner = (part & (sch.splits - 1)) == slice;
+                    if (!owner) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + j * 512), "r"(v[4 * j]),
+                                         "r"(v[4 * j + 1]), "r"(v[4 * j + 2]), "r"(v[4 * j + 3])
+                                         : "memory");
+                    }
+                    cluster_sync_all();
+                    if (!owner) continue;
+                    float sum[32];
+                    for (int s = 0; s < sch.splits; ++s) {
+                        const uint32_t from = mapa_shared(at, s);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            uint4 t = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                            if (s != slice)
+                                asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                             : "=r"(t.x), "=r"(t.y), "=r"(t.z), "=r"(t.w)
+                                             : "r"(from + j * 512));
+                            const float4 f = make_float4(__uint_as_float(t.x), __uint_as_float(t.y), __uint_as_float(t.z),
+                                                         __uint_as_float(t.w));
+                            sum[4 * j] = s ? sum[4 * j] + f.x : f.x;
+                            sum[4 * j + 1] = s ? sum[4 * j + 1] + f.y : f.y;
+                            sum[4 * j + 2] = s ? sum[4 * j + 2] + f.z : f.z;
+                            sum[4 * j + 3] = s ? sum[4 * j + 3] + f.w : f.w;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sum[j]);
                 }
                 if (col >= g.n || row0 >= g.m) continue;       // warp-uniform
                 f2 x[16];
@@ -588,10 +634,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
                 if (kBox == 32) flush(col, row0);
             }
-            if (kBox > 32 && col0 < g.n && row0 < g.m) flush(col0, row0);
+            if (kBox > 32 && owner && col0 < g.n && row0 < g.m) flush(col0, row0);
             if constexpr (kQuantOut) {
                 // scale bytes of this row's blocks: one or two neighbours; zero past m and n
-                if (row0 / 128 < (g.m + 127) / 128 && col0 / 128 < ykt) {
+                if (owner && row0 / 128 < (g.m + 127) / 128 && col0 / 128 < ykt) {
                     uint8_t* p = static_cast<uint8_t*>(g.scales) + scale_offset(row0 + lane, col0 / 32, ykt);
                     if constexpr (kChunks == 2) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(bytes);
                     else *p = static_cast<uint8_t>(bytes);
@@ -603,7 +649,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if constexpr (kPair) cluster_sync_all();   // no CTA leaves while the pair's MMAs may still read its shared memory
+    // no CTA leaves while the pair's MMAs, or the cluster's sums, may still read its shared memory
+    if constexpr (kPair || kSplit) cluster_sync_all();
     if (warp == 0) {
         tc_fence_after();
         if constexpr (kPair)
@@ -630,8 +677,8 @@ bool out_map(CUtensorMap* map, void* p, Elt e, bool quant, int64_t cols, int64_t
               CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <MxFormat F, int BN, bool kPair, typename O, bool kQ>
-cudaError_t launch(const MxGemmArgs& g, cudaStream_t st) {
+template <MxFormat F, int BN, bool kPair, bool kSplit, typename O, bool kQ>
+cudaError_t launch(const MxGemmArgs& g, int splits, cudaStream_t st) {
     using C = Cfg<F, BN, kPair, kQ ? 1 : static_cast<int>(sizeof(O))>;
     CUtensorMap ta, tb, sa, sb;
     const int64_t row_bytes = (static_cast<int64_t>(g.k) * mx_bits(F) + 7) / 8;
@@ -646,18 +693,20 @@ cudaError_t launch(const MxGemmArgs& g, cudaStream_t st) {
     sch.n_tiles = (g.n + BN - 1) / BN;
     sch.ktiles = (g.k + Kind<F>::kElems - 1) / Kind<F>::kElems;
     sch.units = sch.m_tiles * sch.n_tiles;
+    sch.splits = splits;
+    sch.kt_per = (sch.ktiles + splits - 1) / splits;
     sch.per = 8u * sch.n_tiles;
     sch.magic = static_cast<uint32_t>((uint64_t(1) << 32) / sch.per);
     const bool tensor_store = kQ || (g.y_pitch % 16 == 0 && reinterpret_cast<uintptr_t>(g.y) % 16 == 0);
     CUtensorMap ty{};
     if (tensor_store && !out_map(&ty, kQ ? g.codes : g.y, g.out, kQ, kQ ? g.y_pitch : g.n, g.m, g.y_pitch, C::kBox))
         return cudaErrorInvalidValue;
-    auto kern = mx_gemm_kernel<F, BN, kPair, O, kQ>;
+    auto kern = mx_gemm_kernel<F, BN, kPair, kSplit, O, kQ>;
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = allow_smem(kern, allowed, static_cast<int>(C::kSmemBytes));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(kPair ? 2 * std::min(sch.units, num_sms() / 2) : std::min(sch.units, num_sms()));
+    cfg.gridDim = dim3(kSplit ? sch.units * splits : kPair ? 2 * std::min(sch.units, num_sms() / 2) : std::min(sch.units, num_sms()));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = C::kSmemBytes;
     cfg.stream = st;
@@ -665,19 +714,19 @@ cudaError_t launch(const MxGemmArgs& g, cudaStream_t st) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.x = kSplit ? splits : 2;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = kPair ? 2 : 1;
+    cfg.numAttrs = kPair || kSplit ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, ta, tb, sa, sb, ty, g, sch, tensor_store);
 }
 
-template <MxFormat F, int BN, bool kPair>
-cudaError_t by_output(const MxGemmArgs& g, cudaStream_t st) {
-    if (g.codes) return launch<F, BN, kPair, float, true>(g, st);
-    if (g.out == Elt::kBF16) return launch<F, BN, kPair, __nv_bfloat16, false>(g, st);
-    if (g.out == Elt::kF16) return launch<F, BN, kPair, __half, false>(g, st);
-    return launch<F, BN, kPair, float, false>(g, st);
+template <MxFormat F, int BN, bool kPair, bool kSplit>
+cudaError_t by_output(const MxGemmArgs& g, cudaStream_t st, int splits = 1) {
+    if (g.codes) return launch<F, BN, kPair, kSplit, float, true>(g, splits, st);
+    if (g.out == Elt::kBF16) return launch<F, BN, kPair, kSplit, __nv_bfloat16, false>(g, splits, st);
+    if (g.out == Elt::kF16) return launch<F, BN, kPair, kSplit, __half, false>(g, splits, st);
+    return launch<F, BN, kPair, kSplit, float, false>(g, splits, st);
 }
 
 template <MxFormat F>
@@ -689,10 +738,19 @@ cudaError_t by_tile(const MxGemmArgs& g, cudaStream_t st) {
     // and 19.6; 512 x 4096 x 4096: 9.9 and 13.6).
     const int64_t sms = num_sms(), rt = (g.m + 127) / 128;
     const int64_t pairs = (rt + 1) / 2 * ((g.n + 255) / 256);
-    if (g.k >= 8 * Kind<F>::kElems && pairs >= sms) return by_output<F, 256, true>(g, st);
+    if (g.k >= 8 * Kind<F>::kElems && pairs >= sms) return by_output<F, 256, true, false>(g, st);
     const int64_t w128 = (rt * ((g.n + 127) / 128) + sms - 1) / sms, w256 = (rt * ((g.n + 255) / 256) + sms - 1) / sms;
-    if (7 * w256 < 4 * w128) return by_output<F, 256, false>(g, st);
-    return by_output<F, 128, false>(g, st);
+    if (7 * w256 < 4 * w128) return by_output<F, 256, false, false>(g, st);
+    const int64_t tiles = rt * ((g.n + 127) / 128);
+    const int ktiles = (g.k + Kind<F>::kElems - 1) / Kind<F>::kElems;
+    // Slices of a long reduction where the tiles leave SMs idle: the cluster costs 3 us and a stage 0.33 us, so from 24
+    // stages on (one / two / four slices: mxfp8 93 x 301 x 4641 17.7 / 14.4 / 12.8, 48 x 8192 x 8192 20.7 / 16.0 / -,
+    // mxfp4 512 x 1024 x 8192 12.6 / 11.0 / 11.0; nvfp4 128 x 4096 x 4096, 16 stages, 8.5 / 9.0 / 9.7).
+    for (int splits = 4; splits > 1 && ktiles >= 24; splits /= 2) {
+        const int per = (ktiles + splits - 1) / splits;
+        if (tiles * splits <= sms && (splits - 1) * per < ktiles) return by_output<F, 128, false, true>(g, st, splits);
+    }
+    return by_output<F, 128, false, false>(g, st);
 }
 
 }  // namespace

@@ -88,7 +88,8 @@ def _product64(xv, wv, b, act):
 
 
 SIZES = [(1, 1, 1), (1, 64, 64), (2, 130, 32), (7, 128, 111), (17, 2050, 100), (33, 96, 257), (64, 300, 512),
-         (65, 129, 300), (128, 128, 1024), (200, 520, 384), (300, 256, 2000), (2500, 1300, 200)]
+         (65, 129, 300), (128, 128, 1024), (200, 520, 384), (300, 256, 2000), (2500, 1300, 200),
+         (70, 200, 6200), (300, 131, 6500), (40, 1000, 9000)]      # the last three: reductions in slices
 
 
 @pytest.mark.parametrize("fmt", FORMATS)

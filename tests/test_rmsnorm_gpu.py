@@ -12,7 +12,7 @@ UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0
 TINY = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -149}
 EPS = 1e-6
 SHAPES = [(1, 1), (1, 64), (3, 7), (9, 128), (5, 111), (130, 384), (17, 1000), (33, 1024), (6, 2048), (11, 1111),
-          (3, 4096), (2, 5001), (3, 8192), (2, 16384), (2, 16383), (2500, 96)]
+          (3, 4096), (2, 5001), (3, 8192), (2, 16384), (2, 16383), (2500, 96), (1500, 518), (700, 2047), (301, 8190)]
 
 
 def _inputs(rows, dim, dtype, wdtype, seed=0):
