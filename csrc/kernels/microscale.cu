@@ -35,6 +35,7 @@ __global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 4 : 3)
     const int unit = amax ? units - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x);
     const int ct = unit % col_tiles, line = unit / col_tiles;
     float g = 1.f;
+    if (!amax) wait_previous();
     if constexpr (!Tr::kPow2) {
         if (!amax && g_io) g = *g_io;
     }
@@ -50,7 +51,7 @@ __global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 4 : 3)
     }
     if constexpr (!Tr::kPow2) {
         if (amax) {
-            wait_previous();      // for the maximum; x was complete before that pass began
+            wait_previous();      // for the maximum; x was complete before that pass began (an ordinary launch)
             g = tensor_scale(*amax);
             if (unit == 0 && threadIdx.x == 0) *g_io = g;
         }
@@ -239,20 +240,11 @@ cudaError_t launch_mx_quantize(Elt et, MxFormat f, const void* x, int64_t ld, in
         return by_format(f, [&](auto fc) -> cudaError_t {
             constexpr MxFormat F = decltype(fc)::value;
             auto run = [&](auto kern) {
-                cudaLaunchConfig_t cfg{};
-                cfg.gridDim = dim3(static_cast<unsigned>(units));
-                cfg.blockDim = dim3(kQThreads);
-                cfg.stream = st;
-                cudaLaunchAttribute attr;
-                attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-                attr.val.programmaticStreamSerializationAllowed = 1;
-                cfg.attrs = &attr;
-                const uint32_t* found = F == MxFormat::kNvFp4 ? amax : nullptr;
-                cfg.numAttrs = found ? 1 : 0;      // only then does the kernel wait for the one before
-                return cudaLaunchKernelEx(&cfg, kern, static_cast<const T*>(x), ld, rows, dim, static_cast<uint8_t*>(codes),
-                                          mx_pitch(f, dim), static_cast<uint8_t*>(scales),
-                                          static_cast<int>(mx_scale_tiles(f, dim)), static_cast<int>(col_tiles),
-                                          static_cast<int>(units), g, found, align);
+                return launch_early(kern, dim3(static_cast<unsigned>(units)), kQThreads, st, static_cast<const T*>(x), ld,
+                                    rows, dim, static_cast<uint8_t*>(codes), mx_pitch(f, dim),
+                                    static_cast<uint8_t*>(scales), static_cast<int>(mx_scale_tiles(f, dim)),
+                                    static_cast<int>(col_tiles), static_cast<int>(units), g,
+                                    F == MxFormat::kNvFp4 ? amax : nullptr, align);
             };
             if (row_threads == 32) return run(mx_quantize_kernel<T, F, 32>);
             return run(mx_quantize_kernel<T, F, 8>);

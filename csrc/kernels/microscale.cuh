@@ -160,8 +160,11 @@ __device__ __forceinline__ float tensor_scale(uint32_t amax_bits) {
     return fmaxf(a * (1.0f / 2688.0f), 7.888609052210118e-31f);
 }
 
-// Overlap of a quantisation with the set-up of the product that reads it (programmatic dependent launch): the first
-// lets the next kernel start, the second, there, waits until everything launched before is complete.
+// Overlap of a kernel's start with the end of the one before it (programmatic dependent launch).  allow_next lets the
+// next kernel's CTAs start where there is room; wait_previous, before anything that another kernel may have written
+// is read and before anything is written, waits until all that was launched before is complete.
+// Measured back to back in a graph, without and with it: nvfp4 product of 1 x 4096 x 4096 7.6 and 6.0 us, norm to mxfp8
+// of 10400 x 384 7.95 and 7.5, mxfp4 quantisation of 1536 x 384 3.2 and 2.6.
 __device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -317,6 +320,21 @@ __device__ __forceinline__ void store_any_vec(T* p, const uint4& w, int n) {
                 else reinterpret_cast<unsigned short*>(p)[i] = static_cast<unsigned short>(u[i >> 1] >> (16 * (i & 1)));
             }
     }
+}
+
+// Launch of a kernel that calls wait_previous.
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kern)(Params...), dim3 grid, int threads, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...);
 }
 
 // Lets a kernel use `bytes` of dynamic shared memory; asked of each device once (a launch's host time counts).

@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     __syncthreads();
     tc_fence_after();
     wait_previous();
+    allow_next();
     const uint32_t tmem = ctl->tmem_base;
     const uint32_t elected = elect_lane();
 

@@ -364,6 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (kPair) cluster_sync_all();   // the other CTA's barriers are initialised before anything targets them
     tc_fence_after();
     wait_previous();
+    allow_next();
     constexpr uint32_t tmem = 0;                // all 512 columns are this CTA's: they start at 0
 
     if (warp == 0) {

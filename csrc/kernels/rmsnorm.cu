@@ -22,7 +22,7 @@ namespace {
 
 using namespace mx;
 
-constexpr int kRingStages = 8;
+constexpr int kRingStages = 8, kRingBytes = 216 * 1024;
 
 // A vector of a row as loaded: unpacked where it is used, so that a waiting row takes 4 registers per 16 bytes
 // (8 as fp32), which is what decides how many rows an SM has in flight.  `left`: elements of the row from here on.
@@ -127,7 +127,8 @@ template <typename T, bool kAligned, int kGroup, int KV, bool kQuant>
 __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(RmsFwdArgs a) {
     constexpr int VEC = VecOf<T>::kN;
     __shared__ float red[32];
-    if (kQuant) allow_next();
+    allow_next();
+    wait_previous();
     constexpr int kRows = kGroup == 32 ? 8 : 1;
     const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + (kGroup == 32 ? threadIdx.x >> 5 : 0);
     const int t = threadIdx.x & (kGroup - 1);
@@ -509,11 +510,9 @@ cudaError_t launch_rms_fwd(Elt et, const RmsFwdArgs& a, cudaStream_t st) {
                 const int64_t per = G == 32 ? 8 : 1, blocks = (rows + per - 1) / per;
                 if (blocks >= (int64_t(1) << 31)) return cudaErrorInvalidValue;
                 const int threads = G == 32 ? 256 : G;
-                if (quant)
-                    rms_fwd_kernel<T, kAligned, G, KV, true><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
-                else
-                    rms_fwd_kernel<T, kAligned, G, KV, false><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
-                return cudaGetLastError();
+                const dim3 grid(static_cast<unsigned>(blocks));
+                return quant ? launch_early(rms_fwd_kernel<T, kAligned, G, KV, true>, grid, threads, st, a)
+                             : launch_early(rms_fwd_kernel<T, kAligned, G, KV, false>, grid, threads, st, a);
             });
         };
         return whole ? run(std::true_type{}) : run(std::false_type{});
@@ -538,21 +537,24 @@ cudaError_t ring_bwd(const RmsBwdArgs& a, cudaStream_t st) {
     const int vecs = (a.dim + VecOf<T>::kN - 1) / VecOf<T>::kN;
     const int stage = 3 * static_cast<int>(ring_slot<T>(a.dim, kAligned));
     const int per_sm = vecs <= 128 ? 8 : (vecs <= 256 ? 6 : (3 * stage <= 72 * 1024 ? 3 : (2 * stage <= 108 * 1024 ? 2 : 1)));
-    const int stages = std::min(kRingStages, 216 * 1024 / per_sm / stage);
+    const int stages = std::min(kRingStages, kRingBytes / per_sm / stage);
     if (vecs <= 64 || vecs > 2048 || stages < 2) return cudaErrorNotSupported;
     const int blocks = static_cast<int>(std::min<int64_t>(a.rows, static_cast<int64_t>(num_sms()) * per_sm));
-    auto run = [&](auto kern, int threads) -> cudaError_t {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, stages * stage);
+    auto run = [&](auto tc, auto kc) -> cudaError_t {
+        constexpr int kThreads = decltype(tc)::value, KV = decltype(kc)::value;
+        static std::atomic<uint64_t> allowed{0};
+        const cudaError_t e = allow_smem(rms_bwd_ring_kernel<T, kAligned, kThreads, KV>, allowed, kRingBytes);
         if (e != cudaSuccess) return e;
-        kern<<<blocks, threads, stages * stage, st>>>(a, stages);
+        rms_bwd_ring_kernel<T, kAligned, kThreads, KV><<<blocks, kThreads, stages * stage, st>>>(a, stages);
         const cudaError_t l = cudaGetLastError();
         return l != cudaSuccess ? l : sum_gw<T>(a, blocks, st);
     };
-    if (vecs <= 128) return run(rms_bwd_ring_kernel<T, kAligned, 128, 1>, 128);
-    if (vecs <= 256) return run(rms_bwd_ring_kernel<T, kAligned, 128, 2>, 128);
-    if (vecs <= 512) return run(rms_bwd_ring_kernel<T, kAligned, 256, 2>, 256);
-    if (vecs <= 1024) return run(rms_bwd_ring_kernel<T, kAligned, 256, 4>, 256);
-    return run(rms_bwd_ring_kernel<T, kAligned, 512, 4>, 512);
+    using std::integral_constant;
+    if (vecs <= 128) return run(integral_constant<int, 128>{}, integral_constant<int, 1>{});
+    if (vecs <= 256) return run(integral_constant<int, 128>{}, integral_constant<int, 2>{});
+    if (vecs <= 512) return run(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+    if (vecs <= 1024) return run(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+    return run(integral_constant<int, 512>{}, integral_constant<int, 4>{});
 }
 
 template <typename T, bool kAligned>
