@@ -17,18 +17,19 @@ namespace {
 
 using namespace mx;
 
-constexpr int kQThreads = 256;
+constexpr int kQThreads = 256, kAmaxThreads = 1024;
 
 // kRow threads side by side in a row (8 or 32: 128 or 512 columns a CTA, of 4 x 32 or 4 x 8 rows).
 template <typename T, MxFormat F, int kRow>
 __global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 4 : 3)
     mx_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t dim, uint8_t* __restrict__ codes,
                        int64_t pitch, uint8_t* __restrict__ scales, int kt, int col_tiles, int units,
-                       float* __restrict__ g_io, const uint32_t* __restrict__ amax, int align) {
+                       float* __restrict__ g_io, const uint32_t* __restrict__ amax, int parts, int align) {
     using Tr = Traits<F>;
     constexpr int kCols = 16 * kRow, kLines = kQThreads / kRow;      // kLines: values of r % 32
     constexpr int kAtoms = kCols / (4 * Tr::kBlock);                 // scale tiles across a CTA's columns
     __shared__ __align__(16) uint8_t tile[kAtoms * kLines * 16];
+    __shared__ uint32_t warp_max[kQThreads / 32];
     allow_next();
     // with amax the maximum was found by a pass in ascending order just before: going backwards, this pass
     // finds the end of x still in L2
@@ -51,8 +52,15 @@ __global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 4 : 3)
     }
     if constexpr (!Tr::kPow2) {
         if (amax) {
-            wait_previous();      // for the maximum; x was complete before that pass began (an ordinary launch)
-            g = tensor_scale(*amax);
+            wait_previous();      // for the maxima; x was complete before that pass let this one start
+            uint32_t m = 0;
+            for (int i = threadIdx.x; i < parts; i += kQThreads) m = max(m, amax[i]);
+            m = __reduce_max_sync(0xffffffffu, m);
+            if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kQThreads / 32; ++i) m = max(m, warp_max[i]);
+            g = tensor_scale(m);
             if (unit == 0 && threadIdx.x == 0) *g_io = g;
         }
     }
@@ -100,13 +108,15 @@ __device__ __forceinline__ uint32_t amax_bits_of(const uint4& w) {
     return m;
 }
 
-// Largest magnitude of a matrix, as bits (an order that keeps NaN; max does not depend on the order).  A dense one is
-// read as one row.
+// Largest magnitude of each CTA's part of a matrix, as bits (an order that keeps NaN; max does not depend on the order);
+// the pass that reads them takes the largest.  A dense matrix is read as one row.
 template <typename T>
-__global__ void __launch_bounds__(512) mx_amax_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t dim,
+__global__ void __launch_bounds__(kAmaxThreads) mx_amax_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t dim,
                                                       uint32_t* __restrict__ amax) {
     constexpr int kN = VecOf<T>::kN;
+    __shared__ uint32_t warp_max[kAmaxThreads / 32];
     uint32_t m = 0;
+    wait_previous();      // before the next pass may start: it reads x without waiting for this one
     allow_next();
     // CTAs side by side in a row, then over the rows
     const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
@@ -128,7 +138,12 @@ __global__ void __launch_bounds__(512) mx_amax_kernel(const T* __restrict__ x, i
         }
     }
     m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0 && m) atomicMax(amax, m);
+    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    m = threadIdx.x < kAmaxThreads / 32 ? warp_max[threadIdx.x] : 0;
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (threadIdx.x == 0) amax[blockIdx.y * gridDim.x + blockIdx.x] = m;
 }
 
 // 16 values of a lane to an unaligned place: the aligned granules between its vectors whole, the ends in pieces.
@@ -226,15 +241,17 @@ cudaError_t launch_mx_quantize(Elt et, MxFormat f, const void* x, int64_t ld, in
         using T = elt_t;
         const int kN = 16 / static_cast<int>(sizeof(T));
         const int align = row_align(x, ld * static_cast<int64_t>(sizeof(T)));
+        int parts = 0;
         if (f == MxFormat::kNvFp4 && amax) {
-            cudaError_t e = cudaMemsetAsync(amax, 0, sizeof(uint32_t), st);
-            if (e != cudaSuccess) return e;
+            const int64_t most = std::min<int64_t>(2 * num_sms(), kMxAmaxParts);
             const int64_t r = ld == dim ? 1 : rows, d = ld == dim ? rows * dim : dim;
-            const int64_t across = std::max<int64_t>(1, std::min<int64_t>((d + 512 * kN - 1) / (512 * kN), num_sms() * 4));
+            const int64_t across =
+                std::max<int64_t>(1, std::min((d + kAmaxThreads * kN - 1) / (kAmaxThreads * kN), most));
             const dim3 grid(static_cast<unsigned>(across),
-                            static_cast<unsigned>(std::min<int64_t>(r, std::max<int64_t>(1, num_sms() * 4 / across))));
-            mx_amax_kernel<T><<<grid, 512, 0, st>>>(static_cast<const T*>(x), ld, r, d, amax);
-            e = cudaGetLastError();
+                            static_cast<unsigned>(std::min(r, std::max<int64_t>(1, most / across))));
+            parts = static_cast<int>(grid.x * grid.y);
+            const cudaError_t e = launch_early(mx_amax_kernel<T>, grid, kAmaxThreads, st, static_cast<const T*>(x), ld, r,
+                                               d, amax);
             if (e != cudaSuccess) return e;
         }
         return by_format(f, [&](auto fc) -> cudaError_t {
@@ -244,7 +261,7 @@ cudaError_t launch_mx_quantize(Elt et, MxFormat f, const void* x, int64_t ld, in
                                     rows, dim, static_cast<uint8_t*>(codes), mx_pitch(f, dim),
                                     static_cast<uint8_t*>(scales), static_cast<int>(mx_scale_tiles(f, dim)),
                                     static_cast<int>(col_tiles), static_cast<int>(units), g,
-                                    F == MxFormat::kNvFp4 ? amax : nullptr, align);
+                                    F == MxFormat::kNvFp4 ? amax : nullptr, parts, align);
             };
             if (row_threads == 32) return run(mx_quantize_kernel<T, F, 32>);
             return run(mx_quantize_kernel<T, F, 8>);

@@ -17,8 +17,9 @@ constexpr int64_t mx_pitch(MxFormat f, int64_t dim) { return ((dim * mx_bits(f) 
 constexpr int64_t mx_scale_tiles(MxFormat f, int64_t dim) { return (dim + 4 * mx_block(f) - 1) / (4 * mx_block(f)); }
 
 // x [rows, dim] (row pitch ld) -> codes [rows, mx_pitch], scales [ceil(rows / 128), mx_scale_tiles, 512].
-// nvfp4: g (fp32 [1], null: 1) is the tensor's scale; with amax (uint32 [1], work space) g is an output,
+// nvfp4: g (fp32 [1], null: 1) is the tensor's scale; with amax (uint32 [kMxAmaxParts], work space) g is an output,
 // found first.
+constexpr int kMxAmaxParts = 512;
 cudaError_t launch_mx_quantize(Elt et, MxFormat f, const void* x, int64_t ld, int64_t rows, int64_t dim, void* codes,
                                void* scales, float* g, uint32_t* amax, cudaStream_t st);
 cudaError_t launch_mx_dequantize(Elt et, MxFormat f, const void* codes, const void* scales, const float* g,

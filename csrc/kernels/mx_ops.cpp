@@ -135,7 +135,7 @@ std::vector<OptTensor> mx_quantize(torch::Tensor x, int64_t fmt, OptTensor g) {
         } else {
             gt = rows ? fresh({1}, torch::kFloat32, x)
                       : torch::ones({1}, x.options().dtype(torch::kFloat32));
-            work.emplace(sizeof(uint32_t));
+            work.emplace(kMxAmaxParts * sizeof(uint32_t));
         }
     } else {
         TORCH_CHECK(!has(g), "mx_quantize: only nvfp4 has a tensor scale");
