@@ -7,8 +7,10 @@
 // r + 96: the four loads are in flight together, held as loaded, and the four rows' scale bytes are
 // neighbours in their tile.  The tiles' rows are put together in shared memory and leave as whole
 // sectors; a tile built from byte stores of CTAs that run at different times would reach DRAM in parts.
-// Measured, 16384 x 8192 bf16: mxfp4 52 us (6.5 TB/s), nvfp4 54 us, with the tensor's scale found first 99 us,
-// mxfp8 60 us; back to bf16 64 us (5.3 TB/s).
+// Measured, 16384 x 8192 bf16: mxfp4 52 us (6.5 TB/s), nvfp4 54 us, with the tensor's scale found first 97 us,
+// mxfp8 60 us; back to bf16 64 us (5.3 TB/s).  fp32: mxfp4 89 us, nvfp4 93 (105 at three CTAs an SM, which spill),
+// mxfp8 97.  1536 x 384: 2.6 us, nvfp4 with its scale found 4.8.  Reading all but the end of x past L2 in the pass for
+// the scale (for the second pass to find more there) changed nothing: 97 and 97 us.
 #include "microscale.cuh"
 
 namespace mmltk {
@@ -21,7 +23,7 @@ constexpr int kQThreads = 256, kAmaxThreads = 1024;
 
 // kRow threads side by side in a row (8 or 32: 128 or 512 columns a CTA, of 4 x 32 or 4 x 8 rows).
 template <typename T, MxFormat F, int kRow>
-__global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 4 : 3)
+__global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 4 : 2)
     mx_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t dim, uint8_t* __restrict__ codes,
                        int64_t pitch, uint8_t* __restrict__ scales, int kt, int col_tiles, int units,
                        float* __restrict__ g_io, const uint32_t* __restrict__ amax, int parts, int align) {
