@@ -27,11 +27,14 @@
 // registers took as long as the rest of a short product together).  The quantised output (mxfp8) needs
 // no second pass: a thread has 32 consecutive columns of a row, one scale block.
 //
-// Measured (B200, CUDA-graph replays): 8192^3 mxfp8 375 us (2.9 PFLOP/s), mxfp4 197 us (5.6), nvfp4 222 us (5.0).  These
+// Few tiles and a long reduction: the CTAs of a cluster each take a slice of it, leave their partial sums in
+// their (now free) stages, and after a cluster barrier each finishes a part of the columns, adding the slices in order.
+//
+// Measured (B200, CUDA-graph replays): 8192^3 mxfp8 370 us (2.9 PFLOP/s), mxfp4 197 us (5.6), nvfp4 222 us (5.0).  These
 // run at the power cap (1.35 to 1.55 GHz; a bf16 cuBLAS product there 1.1 PFLOP/s); the tensor pipe is busy
 // 74 % of the cycles (4096^3 mxfp8).  nvfp4 is slower than mxfp4 by its scale copies: 12 a stage take 132
 // cycles beside the MMAs' 512, 6 take 52, 3 none.  Short products are bound by issue slots: at
-// 31200 x 2048 x 256 to mxfp8 (30 us; 66 MB out, 10 us) the epilogue's warps use 58 % of them, and the
+// 31200 x 2048 x 256 to mxfp8 (29 us; 66 MB out, 10 us) the epilogue's warps use 58 % of them, and the
 // scheduler keeps a ready warp going, so the issuing warp waits for the epilogue's bursts.
 //
 // Every wait is bounded: on a time-out the kernel records which role gave up in a status word and

@@ -10,7 +10,7 @@
 // elements, a CTA of 128 to 512 threads beyond -- so every element is read once; statistics are
 // fp32.  A thread's elements are 16-byte vectors kGroup vectors apart, so the 2 to 8 threads of a
 // scale block are neighbours in a warp and find its maximum with at most three shuffles.
-// Measured, bf16 with a residual: forward 32768 x 4096 159 us (6.8 TB/s), to mxfp8 141 us (6.7 TB/s); backward
+// Measured, bf16 with a residual: forward 32768 x 4096 157 us (6.8 TB/s), to mxfp8 139 us (6.8 TB/s); backward
 // 166 us (6.5 TB/s); 16384 x 8191, whose rows start anywhere, 303, 288 and 328 us (16384 x 8192: 159, 146, 171): the
 // narrow stores bound those.
 #include "microscale.cuh"
