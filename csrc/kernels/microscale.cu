@@ -252,14 +252,14 @@ cudaError_t launch_mx_quantize(Elt et, MxFormat f, const void* x, int64_t ld, in
             const dim3 grid(static_cast<unsigned>(across),
                             static_cast<unsigned>(std::min(r, std::max<int64_t>(1, most / across))));
             parts = static_cast<int>(grid.x * grid.y);
-            const cudaError_t e = launch_early(mx_amax_kernel<T>, grid, kAmaxThreads, st, static_cast<const T*>(x), ld, r,
+            const cudaError_t e = launch_early(mx_amax_kernel<T>, grid, kAmaxThreads, st, 0, static_cast<const T*>(x), ld, r,
                                                d, amax);
             if (e != cudaSuccess) return e;
         }
         return by_format(f, [&](auto fc) -> cudaError_t {
             constexpr MxFormat F = decltype(fc)::value;
             auto run = [&](auto kern) {
-                return launch_early(kern, dim3(static_cast<unsigned>(units)), kQThreads, st, static_cast<const T*>(x), ld,
+                return launch_early(kern, dim3(static_cast<unsigned>(units)), kQThreads, st, 0, static_cast<const T*>(x), ld,
                                     rows, dim, static_cast<uint8_t*>(codes), mx_pitch(f, dim),
                                     static_cast<uint8_t*>(scales), static_cast<int>(mx_scale_tiles(f, dim)),
                                     static_cast<int>(col_tiles), static_cast<int>(units), g,

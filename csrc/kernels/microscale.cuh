@@ -324,10 +324,11 @@ __device__ __forceinline__ void store_any_vec(T* p, const uint4& w, int n) {
 
 // Launch of a kernel that calls wait_previous.
 template <typename... Params, typename... Args>
-cudaError_t launch_early(void (*kern)(Params...), dim3 grid, int threads, cudaStream_t st, Args... args) {
+cudaError_t launch_early(void (*kern)(Params...), dim3 grid, int threads, cudaStream_t st, int smem, Args... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

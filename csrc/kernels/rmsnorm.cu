@@ -11,8 +11,8 @@
 // fp32.  A thread's elements are 16-byte vectors kGroup vectors apart, so the 2 to 8 threads of a
 // scale block are neighbours in a warp and find its maximum with at most three shuffles.
 // Measured, bf16 with a residual: forward 32768 x 4096 157 us (6.8 TB/s), to mxfp8 139 us (6.8 TB/s); backward
-// 166 us (6.5 TB/s); 16384 x 8191, whose rows start anywhere, 303, 288 and 328 us (16384 x 8192: 159, 146, 171): the
-// narrow stores bound those.
+// 166 us (6.5 TB/s); 16384 x 7001, whose rows start anywhere, 145 and 175 us (at the copy's rate 140 and
+// 123), its backward without a residual 162 (105).
 #include "microscale.cuh"
 #include "tcgen05.cuh"
 
@@ -24,46 +24,93 @@ using namespace mx;
 
 constexpr int kRingStages = 8, kRingBytes = 216 * 1024;
 
+// Where the rows start.  kWhole: every row on a 16-byte boundary.  kPhase: anywhere, but row r of every tensor equally far
+// past one (dense tensors of any width): the vectors are then the aligned granules of a row, the first one reaching
+// `lead` elements before it and the last one behind it, and only the weights have to be shifted.  kAny: each
+// tensor in its own way; vectors start with the row, are read in aligned granules and shifted, and are written
+// in the widest pieces the address allows.  bf16 with a residual, us as kAny and kPhase:
+// 16384 x 7001 forward 261 and 145, to mxfp8 256 and 175, backward 263 and 162; 32768 x 518 42 and 38, 51 and 46, 76 and 69.
+enum Rows { kWhole, kPhase, kAny };
+
 // A vector of a row as loaded: unpacked where it is used, so that a waiting row takes 4 registers per 16 bytes
-// (8 as fp32), which is what decides how many rows an SM has in flight.  `left`: elements of the row from here on.
-// Rows that start anywhere (kAligned = false: a width or pitch that is no multiple of 16 bytes) are read in
-// aligned granules and shifted, and written in the widest pieces the address allows.
-template <typename T, bool kAligned>
+// (8 as fp32), which is what decides how many rows an SM has in flight.  i: its first element in the row (below 0 for
+// kPhase's first one), below dim.  Elements outside the row read as zeros and are not written.
+template <typename T, Rows kRows>
 struct Raw {
+    static constexpr int kN = VecOf<T>::kN;
     uint4 w;
-    __device__ __forceinline__ void load(const T* p, int left) {
-        if constexpr (kAligned) w = *reinterpret_cast<const uint4*>(p);
-        else w = load_any(p, min(left, VecOf<T>::kN));
+    __device__ __forceinline__ void load(const T* row, int i, int dim) {
+        if constexpr (kRows == kAny) {
+            w = load_any(row + i, min(dim - i, kN));
+        } else {
+            w = *reinterpret_cast<const uint4*>(row + i);
+        }
     }
-    __device__ __forceinline__ void store(T* p, int left) const {
-        if constexpr (kAligned) *reinterpret_cast<uint4*>(p) = w;
-        else store_any_vec(p, w, min(left, VecOf<T>::kN));
+    // kPhase: zeros outside the row; called when all of a row's loads have been issued, since it waits for one
+    __device__ __forceinline__ void trim(int i, int dim) {
+        if constexpr (kRows == kPhase) {
+            if (i < 0 || i + kN > dim) {
+                uint32_t* u = &w.x;
+#pragma unroll
+                for (int e = 0; e < kN; ++e)
+                    if (i + e < 0 || i + e >= dim) {
+                        if constexpr (sizeof(T) == 4) u[e] = 0;
+                        else u[e / 2] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+                    }
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* row, int i, int dim) const {
+        if constexpr (kRows == kAny) {
+            store_any_vec(row + i, w, min(dim - i, kN));
+        } else if (kRows == kWhole || (i >= 0 && i + kN <= dim)) {
+            *reinterpret_cast<uint4*>(row + i) = w;
+        } else if (i >= 0 || i + kN <= dim) {
+            constexpr int kSize = sizeof(T);
+            store_part(reinterpret_cast<char*>(row + i), w, i < 0 ? -i * kSize : 0, min(kN, dim - i) * kSize);
+        } else {      // a row inside one granule
+            store_any_vec(row, shift16(w, make_uint4(0, 0, 0, 0), -i * static_cast<int>(sizeof(T))), dim);
+        }
     }
     __device__ __forceinline__ void get(float* f) const { unpack16(w, f, T()); }
     __device__ __forceinline__ void set(const float* f) { w = pack16(f, T()); }
     __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
 };
 
-// weights (16-byte aligned): x's type or fp32; zeros past the row
-template <typename T, bool kAligned>
-__device__ __forceinline__ void load_w(const void* w, bool f32, int i, int left, float* f) {
+// Weights of x's type at any element i: the two granules, loaded, and shifted where they are used.  Elements outside the
+// row are arbitrary.
+template <typename T>
+struct RawPair {
+    uint4 a, b;
+    __device__ __forceinline__ void load(const T* w, int i, int dim, int sh) {      // w + i is sh bytes past a granule
+        const int at = i * static_cast<int>(sizeof(T)) - sh, end = dim * static_cast<int>(sizeof(T));
+        const char* p = reinterpret_cast<const char*>(w) + at;
+        a = at >= 0 && at < end ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+        b = sh && at + 16 < end ? *reinterpret_cast<const uint4*>(p + 16) : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void get(float* f, int sh) const { unpack16(shift16(a, b, sh), f, T()); }
+};
+
+// weights (16-byte aligned): x's type or fp32; zeros outside the row
+template <typename T, Rows kRows>
+__device__ __forceinline__ void load_w(const void* w, bool f32, int i, int dim, float* f) {
     constexpr int kN = VecOf<T>::kN;
-    if (!kAligned && left < kN) {
+    if (kRows != kWhole && (i < 0 || i + kN > dim)) {
 #pragma unroll
         for (int e = 0; e < kN; ++e)
-            f[e] = e >= left ? 0.f : f32 ? static_cast<const float*>(w)[i + e] : to_f(static_cast<const T*>(w)[i + e]);
+            f[e] = i + e < 0 || i + e >= dim ? 0.f
+                   : f32                     ? static_cast<const float*>(w)[i + e]
+                                             : to_f(static_cast<const T*>(w)[i + e]);
     } else if (f32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(w) + i);
+        const float* p = static_cast<const float*>(w) + i;
 #pragma unroll
-        for (int e = 0; e < kN / 4; ++e) {
-            const float4 t = p[e];
-            f[4 * e] = t.x;
-            f[4 * e + 1] = t.y;
-            f[4 * e + 2] = t.z;
-            f[4 * e + 3] = t.w;
+        for (int e = 0; e < kN; e += 4) {
+            const uint4 t = kRows == kPhase ? load_any(p + e, 4) : *reinterpret_cast<const uint4*>(p + e);
+            unpack16(t, f + e, float());
         }
     } else {
-        unpack16(*reinterpret_cast<const uint4*>(static_cast<const T*>(w) + i), f, T());
+        const T* p = static_cast<const T*>(w) + i;
+        unpack16(kRows == kPhase ? load_any(p, kN) : *reinterpret_cast<const uint4*>(p), f, T());
     }
 }
 
@@ -123,15 +170,18 @@ __device__ __forceinline__ void quantize_store(const float* v, int i, int64_t r,
         *reinterpret_cast<uint32_t*>(scales + scale_offset(r, i / Tr::kBlock, kt)) = b;
 }
 
-template <typename T, bool kAligned, int kGroup, int KV, bool kQuant>
-__global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(RmsFwdArgs a) {
+template <typename T, Rows kRows, int kGroup, int KV, bool kQuant>
+__global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup,
+                                  KV <= 4 ? 1024 / (kGroup == 32 ? 256 : kGroup) : 1)
+    rms_fwd_kernel(RmsFwdArgs a) {
     constexpr int VEC = VecOf<T>::kN;
     __shared__ float red[32];
+    extern __shared__ uint4 granules[];
     allow_next();
     wait_previous();
-    constexpr int kRows = kGroup == 32 ? 8 : 1;
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + (kGroup == 32 ? threadIdx.x >> 5 : 0);
-    const int t = threadIdx.x & (kGroup - 1);
+    constexpr int kPer = kGroup == 32 ? 8 : 1;
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * kPer + (kGroup == 32 ? threadIdx.x >> 5 : 0);
+    const int t = kGroup == 32 ? threadIdx.x & 31 : threadIdx.x;
     const int kt = kQuant ? static_cast<int>(mx_scale_tiles(a.fmt, a.dim)) : 0;
     if (r >= a.rows) {   // (all of the row's threads) rows that fill the last scale tile: zero scales
         if (kQuant && r < (a.rows + 127) / 128 * 128)
@@ -139,27 +189,37 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(Rm
                 *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.scales) + scale_offset(r, 4 * i, kt)) = 0;
         return;
     }
+    [[maybe_unused]] uint4* buf = granules + (kGroup == 32 ? threadIdx.x >> 5 : 0) * KV * kGroup;
     const T* xr = static_cast<const T*>(a.x) + r * a.ldx;
     const T* rr = a.res ? static_cast<const T*>(a.res) + r * a.ldr : nullptr;
-    Raw<T, kAligned> v[KV];
+    const int lead = kRows == kPhase ? static_cast<int>(r * a.dim % VEC) : 0;
+    Raw<T, kRows> v[KV];
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
-        const int i = (k * kGroup + t) * VEC;
-        if (i < a.dim) v[k].load(xr + i, a.dim - i);
+        const int i = (k * kGroup + t) * VEC - lead;
+        if (i < a.dim) v[k].load(xr, i, a.dim);
         else v[k].zero();
     }
+    auto trim = [&](Raw<T, kRows>(&row)[KV]) {
+        if constexpr (kRows == kPhase)
+#pragma unroll
+            for (int k = 0; k < KV; ++k) row[k].trim((k * kGroup + t) * VEC - lead, a.dim);
+    };
     float s = 0.f;
     if (rr) {
         T* hr = static_cast<T*>(a.h) + r * a.dim;
-        Raw<T, kAligned> u[KV];
+        Raw<T, kRows> u[KV];
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
-            const int i = (k * kGroup + t) * VEC;
-            if (i < a.dim) u[k].load(rr + i, a.dim - i);
+            const int i = (k * kGroup + t) * VEC - lead;
+            if (i < a.dim) u[k].load(rr, i, a.dim);
+            else u[k].zero();
         }
+        trim(v);
+        trim(u);
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
-            const int i = (k * kGroup + t) * VEC;
+            const int i = (k * kGroup + t) * VEC - lead;
             if (i < a.dim) {
                 // the norm sees the sum as it is stored, so that its backward can start from h
                 float f[VEC], e[VEC];
@@ -168,9 +228,11 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(Rm
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) f[j] += e[j];
                 v[k].set(f);
-                v[k].store(hr + i, a.dim - i);
+                v[k].store(hr, i, a.dim);
             }
         }
+    } else {
+        trim(v);
     }
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
@@ -179,26 +241,47 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(Rm
 #pragma unroll
         for (int j = 0; j < VEC; ++j) s = fmaf(f[j], f[j], s);
     }
+    if constexpr (kQuant && kRows == kPhase) {      // the blocks start with the row: the granules meet in shared memory
+#pragma unroll
+        for (int k = 0; k < KV; ++k) buf[k * kGroup + t] = v[k].w;
+        if constexpr (kGroup == 32) __syncwarp();
+    }
     s = group_sum<kGroup>(s, red);
     const float rstd = 1.f / sqrtf(s / static_cast<float>(a.dim) + a.eps);
     if (a.rstd && t == 0) a.rstd[r] = rstd;
     const int span = kQuant ? kt * 4 * mx_block(a.fmt) : a.dim;
     float g = 1.f;
     if (kQuant && a.g) g = *a.g;
+    const int shift = kQuant ? 0 : lead;
+    // kPhase: weights of x's type, two vectors' on their way before the first is shifted
+    constexpr bool kPairs = kRows == kPhase && !kQuant;
+    const bool pairs = kPairs && (sizeof(T) == 4 || !a.w_f32);
+    const int wsh = lead ? 16 - lead * static_cast<int>(sizeof(T)) : 0;
+    RawPair<T> wp[2];
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
-        const int i = (k * kGroup + t) * VEC;
+        const int i = (k * kGroup + t) * VEC - shift;
+        if (kPairs && pairs && k % 2 == 0) {
+#pragma unroll
+            for (int u = 0; u < (KV - k < 2 ? 1 : 2); ++u)
+                wp[u].load(static_cast<const T*>(a.w), i + u * kGroup * VEC, a.dim, wsh);
+        }
+        if constexpr (kQuant && kRows == kPhase) {      // (after group_sum's barrier)
+            const int j = k * kGroup + t;
+            if (lead) v[k].w = shift16(buf[j], j + 1 < KV * kGroup ? buf[j + 1] : make_uint4(0, 0, 0, 0), lead * sizeof(T));
+        }
         float f[VEC];
         v[k].get(f);
         if (i < a.dim) {
             float w[VEC];
-            load_w<T, kAligned>(a.w, a.w_f32, i, a.dim - i, w);
+            if (kPairs && pairs) wp[k % 2].get(w, wsh);
+            else load_w<T, kQuant && kRows == kPhase ? kAny : kRows>(a.w, a.w_f32, i, a.dim, w);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) f[j] = f[j] * rstd * w[j];
             if constexpr (!kQuant) {
-                Raw<T, kAligned> y;
+                Raw<T, kRows> y;
                 y.set(f);
-                y.store(static_cast<T*>(a.y) + r * a.dim + i, a.dim - i);
+                y.store(static_cast<T*>(a.y) + r * a.dim, i, a.dim);
             }
         }
         if constexpr (kQuant) {
@@ -219,10 +302,10 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup) rms_fwd_kernel(Rm
 // ---------------------------------------------------------------- backward
 // Persistent: a group of threads walks rows and keeps its columns' part of gw in registers; one partial
 // row per CTA, summed in a fixed order by rms_gw_kernel (no atomics: the same bits every run).
-template <typename T, bool kAligned, int kGroup, int KV>
+template <typename T, Rows kRows, int kGroup, int KV>
 __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 : 1) rms_bwd_kernel(RmsBwdArgs a) {
     constexpr int VEC = VecOf<T>::kN;
-    constexpr int kRows = kGroup == 32 ? 8 : 1;
+    constexpr int kPer = kGroup == 32 ? 8 : 1;
     __shared__ float red[2][32];
     __shared__ float part[kGroup == 32 ? 8 * 32 * VEC : 1];
     const int sub = kGroup == 32 ? threadIdx.x >> 5 : 0;
@@ -234,17 +317,17 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 
         for (int e = 0; e < VEC; ++e) acc[k][e] = 0.f;
     const float inv_dim = 1.f / static_cast<float>(a.dim);
     int turn = 0;
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + sub; r < a.rows;
-         r += static_cast<int64_t>(gridDim.x) * kRows, turn ^= 1) {
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kPer + sub; r < a.rows;
+         r += static_cast<int64_t>(gridDim.x) * kPer, turn ^= 1) {
         const float rstd = a.rstd[r];
-        Raw<T, kAligned> hv[KV], gv[KV], ev[KV];
+        Raw<T, kRows> hv[KV], gv[KV], ev[KV];
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
             const int i = (k * kGroup + t) * VEC;
             if (i < a.dim) {
-                hv[k].load(static_cast<const T*>(a.h) + r * a.ldh + i, a.dim - i);
-                gv[k].load(static_cast<const T*>(a.gy) + r * a.ldgy + i, a.dim - i);
-                if (a.gh) ev[k].load(static_cast<const T*>(a.gh) + r * a.ldgh + i, a.dim - i);
+                hv[k].load(static_cast<const T*>(a.h) + r * a.ldh, i, a.dim);
+                gv[k].load(static_cast<const T*>(a.gy) + r * a.ldgy, i, a.dim);
+                if (a.gh) ev[k].load(static_cast<const T*>(a.gh) + r * a.ldgh, i, a.dim);
             }
         }
         float s = 0.f;
@@ -253,7 +336,7 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 
             const int i = (k * kGroup + t) * VEC;
             if (i < a.dim) {
                 float w[VEC], h[VEC], g[VEC];
-                load_w<T, kAligned>(a.w, a.w_f32, i, a.dim - i, w);
+                load_w<T, kRows>(a.w, a.w_f32, i, a.dim, w);
                 hv[k].get(h);
                 gv[k].get(g);
 #pragma unroll
@@ -270,7 +353,7 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 
             const int i = (k * kGroup + t) * VEC;
             if (i < a.dim) {
                 float w[VEC], h[VEC], g[VEC];
-                load_w<T, kAligned>(a.w, a.w_f32, i, a.dim - i, w);
+                load_w<T, kRows>(a.w, a.w_f32, i, a.dim, w);
                 hv[k].get(h);
                 gv[k].get(g);
 #pragma unroll
@@ -281,7 +364,7 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 
                     for (int e = 0; e < VEC; ++e) g[e] += h[e];
                 }
                 hv[k].set(g);
-                hv[k].store(static_cast<T*>(a.gx) + r * a.dim + i, a.dim - i);
+                hv[k].store(static_cast<T*>(a.gx) + r * a.dim, i, a.dim);
             }
         }
     }
@@ -322,7 +405,7 @@ __host__ __device__ constexpr uint32_t ring_slot(int dim, bool aligned) {
     return aligned ? bytes : (bytes + 15) / 16 * 16 + 16;
 }
 
-template <typename T, bool kAligned, int kThreads, int KV>
+template <typename T, Rows kRows, int kThreads, int KV>
 __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, int stages) {
     constexpr int VEC = VecOf<T>::kN;
     extern __shared__ __align__(128) unsigned char ring[];
@@ -330,9 +413,11 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
     __shared__ uint64_t full[kRingStages];
     __shared__ int abort;
     const int t = threadIdx.x;
-    const uint32_t row_bytes = static_cast<uint32_t>(a.dim) * sizeof(T), slot = ring_slot<T>(a.dim, kAligned);
+    const uint32_t row_bytes = static_cast<uint32_t>(a.dim) * sizeof(T), slot = ring_slot<T>(a.dim, kRows == kWhole);
     const int inputs = a.gh ? 3 : 2;
     const int64_t first = blockIdx.x, step = gridDim.x;
+    // (kPhase: the rows of a CTA are a multiple of VEC apart, so its columns and weights stay the same)
+    const int lead = kRows == kPhase ? static_cast<int>(first * a.dim % VEC) : 0;
     const int count = first < a.rows ? static_cast<int>((a.rows - 1 - first) / step) + 1 : 0;
     if (t == 0) {
         for (int s = 0; s < stages; ++s) tc::mbar_init(&full[s], 1);
@@ -353,7 +438,7 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
         uint32_t bytes[3], all = 0;
 #pragma unroll
         for (int i = 0; i < 3; ++i) {      // whole 16-byte granules
-            bytes[i] = kAligned ? row_bytes : (static_cast<uint32_t>(src[i] & 15) + row_bytes + 15) & ~15u;
+            bytes[i] = kRows == kWhole ? row_bytes : (static_cast<uint32_t>(src[i] & 15) + row_bytes + 15) & ~15u;
             if (i < inputs) all += bytes[i];
         }
         tc::mbar_expect_tx(&full[s], all);
@@ -370,10 +455,10 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
     float acc[KV][VEC], w[KV][VEC];
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
-        const int i = (k * kThreads + t) * VEC;
+        const int i = (k * kThreads + t) * VEC - lead;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[k][e] = w[k][e] = 0.f;
-        if (i < a.dim) load_w<T, kAligned>(a.w, a.w_f32, i, a.dim - i, w[k]);
+        if (i < a.dim) load_w<T, kRows>(a.w, a.w_f32, i, a.dim, w[k]);
     }
     const float inv_dim = 1.f / static_cast<float>(a.dim);
     for (int j = 0; j < count; ++j) {
@@ -384,17 +469,19 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
         const T* in[3];
 #pragma unroll
         for (int i = 0; i < 3; ++i)
-            in[i] = reinterpret_cast<const T*>(ring + (s * 3 + i) * slot + (kAligned ? 0 : start(i, r) & 15));
+            in[i] = reinterpret_cast<const T*>(ring + (s * 3 + i) * slot + (kRows == kWhole ? 0 : start(i, r) & 15));
         float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
-            const int i = (k * kThreads + t) * VEC;
+            const int i = (k * kThreads + t) * VEC - lead;
             if (i < a.dim) {
                 float h[VEC], g[VEC];
-                Raw<T, kAligned> v;
-                v.load(in[0] + i, a.dim - i);
+                Raw<T, kRows> v;
+                v.load(in[0], i, a.dim);
+                v.trim(i, a.dim);
                 v.get(h);
-                v.load(in[1] + i, a.dim - i);
+                v.load(in[1], i, a.dim);
+                v.trim(i, a.dim);
                 v.get(g);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
@@ -413,24 +500,27 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
         const float c = sum * inv_dim * rstd * rstd * rstd;
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
-            const int i = (k * kThreads + t) * VEC;
+            const int i = (k * kThreads + t) * VEC - lead;
             if (i < a.dim) {
                 float h[VEC], g[VEC];
-                Raw<T, kAligned> v;
-                v.load(in[0] + i, a.dim - i);
+                Raw<T, kRows> v;
+                v.load(in[0], i, a.dim);
+                v.trim(i, a.dim);
                 v.get(h);
-                v.load(in[1] + i, a.dim - i);
+                v.load(in[1], i, a.dim);
+                v.trim(i, a.dim);
                 v.get(g);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) g[e] = fmaf(rstd, g[e] * w[k][e], -c * h[e]);
                 if (a.gh) {
-                    v.load(in[2] + i, a.dim - i);
+                    v.load(in[2], i, a.dim);
+                    v.trim(i, a.dim);
                     v.get(h);
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) g[e] += h[e];
                 }
                 v.set(g);
-                v.store(static_cast<T*>(a.gx) + r * a.dim + i, a.dim - i);
+                v.store(static_cast<T*>(a.gx) + r * a.dim, i, a.dim);
             }
         }
     }
@@ -438,8 +528,12 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
     float* dst = a.partial + static_cast<int64_t>(blockIdx.x) * rms_partial_pitch(a.dim);
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
-        const int i = (k * kThreads + t) * VEC;
-        if (i < a.dim) {
+        const int i = (k * kThreads + t) * VEC - lead;
+        if (kRows == kPhase) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (i + e >= 0 && i + e < a.dim) dst[i + e] = acc[k][e];
+        } else if (i < a.dim) {
 #pragma unroll
             for (int e = 0; e < VEC; e += 4)
                 *reinterpret_cast<float4*>(dst + i + e) = make_float4(acc[k][e], acc[k][e + 1], acc[k][e + 2], acc[k][e + 3]);
@@ -470,8 +564,8 @@ __global__ void __launch_bounds__(256) rms_gw_kernel(const float* __restrict__ p
 }
 
 // Threads per row and vectors per thread for rows of `vecs` 16-byte vectors: the smallest group that holds them, a
-// warp while a thread keeps at most 4.
-template <bool kLong, typename Fn>
+// warp while a thread keeps at most 4.  kMore: sizes for widths of one vector more than a power of two (kPhase).
+template <bool kLong, bool kMore, typename Fn>
 cudaError_t by_width(int vecs, Fn&& fn) {
 #define MMLTK_RMS_WIDTH(G, KV) \
     if (vecs <= G * KV) return fn(std::integral_constant<int, G>{}, std::integral_constant<int, KV>{})
@@ -480,8 +574,11 @@ cudaError_t by_width(int vecs, Fn&& fn) {
     MMLTK_RMS_WIDTH(32, 4);
     MMLTK_RMS_WIDTH(128, 2);
     MMLTK_RMS_WIDTH(128, 4);
+    if constexpr (kMore) MMLTK_RMS_WIDTH(192, 3);
     MMLTK_RMS_WIDTH(256, 4);
+    if constexpr (kMore) MMLTK_RMS_WIDTH(384, 3);
     MMLTK_RMS_WIDTH(512, 4);
+    if constexpr (kLong && kMore) MMLTK_RMS_WIDTH(768, 3);
     if constexpr (kLong) MMLTK_RMS_WIDTH(512, 8);      // fp32
 #undef MMLTK_RMS_WIDTH
     return cudaErrorInvalidValue;
@@ -503,19 +600,27 @@ cudaError_t launch_rms_fwd(Elt et, const RmsFwdArgs& a, cudaStream_t st) {
         if (!aligned(a.w)) return cudaErrorInvalidValue;
         const bool whole = a.dim % kN == 0 && a.ldx % kN == 0 && aligned(a.x) &&
                            (!a.res || (a.ldr % kN == 0 && aligned(a.res)));
-        auto run = [&](auto ac) -> cudaError_t {
-            constexpr bool kAligned = decltype(ac)::value;
-            return by_width<sizeof(T) == 4>((elems + kN - 1) / kN, [&](auto gc, auto kc) -> cudaError_t {
+        const bool phase = (a.ldx - a.dim) % kN == 0 && aligned(a.x) && (!a.res || ((a.ldr - a.dim) % kN == 0 && aligned(a.res)));
+        auto run = [&](auto mode) -> cudaError_t {
+            constexpr Rows kRows = decltype(mode)::value;
+            const int vecs = (elems + kN - 1) / kN + (kRows == kPhase);
+            return by_width<sizeof(T) == 4, kRows == kPhase>(vecs, [&](auto gc, auto kc) -> cudaError_t {
                 constexpr int G = decltype(gc)::value, KV = decltype(kc)::value;
                 const int64_t per = G == 32 ? 8 : 1, blocks = (rows + per - 1) / per;
                 if (blocks >= (int64_t(1) << 31)) return cudaErrorInvalidValue;
                 const int threads = G == 32 ? 256 : G;
                 const dim3 grid(static_cast<unsigned>(blocks));
-                return quant ? launch_early(rms_fwd_kernel<T, kAligned, G, KV, true>, grid, threads, st, a)
-                             : launch_early(rms_fwd_kernel<T, kAligned, G, KV, false>, grid, threads, st, a);
+                if (!quant) return launch_early(rms_fwd_kernel<T, kRows, G, KV, false>, grid, threads, st, 0, a);
+                constexpr int kSmem = kRows == kPhase ? (G == 32 ? 256 : G) * KV * 16 : 0;
+                constexpr auto kern = rms_fwd_kernel<T, kRows, G, KV, true>;
+                static std::atomic<uint64_t> allowed{0};
+                const cudaError_t e = kSmem > 48 * 1024 ? allow_smem(kern, allowed, kSmem) : cudaSuccess;
+                return e != cudaSuccess ? e : launch_early(kern, grid, threads, st, kSmem, a);
             });
         };
-        return whole ? run(std::true_type{}) : run(std::false_type{});
+        if (whole) return run(std::integral_constant<Rows, kWhole>{});
+        if (phase && (elems + kN - 1) / kN < kRmsMaxDim / kN) return run(std::integral_constant<Rows, kPhase>{});
+        return run(std::integral_constant<Rows, kAny>{});
     });
 }
 
@@ -532,20 +637,22 @@ cudaError_t sum_gw(const RmsBwdArgs& a, int blocks, cudaStream_t st) {
 // barriers of one row are then under other rows' loads (16384 x 8192: 171 us with two CTAs of two stages, 189 with one
 // of four; 65536 x 1024: 101 with eight CTAs, 123 with four).  Not for fp32 rows of over 9000 elements, whose two
 // stages would not fit.
-template <typename T, bool kAligned>
+template <typename T, Rows kRows>
 cudaError_t ring_bwd(const RmsBwdArgs& a, cudaStream_t st) {
-    const int vecs = (a.dim + VecOf<T>::kN - 1) / VecOf<T>::kN;
-    const int stage = 3 * static_cast<int>(ring_slot<T>(a.dim, kAligned));
+    const int vecs = (a.dim + VecOf<T>::kN - 1) / VecOf<T>::kN + (kRows == kPhase);
+    const int stage = 3 * static_cast<int>(ring_slot<T>(a.dim, kRows == kWhole));
     const int per_sm = vecs <= 128 ? 8 : (vecs <= 256 ? 6 : (3 * stage <= 72 * 1024 ? 3 : (2 * stage <= 108 * 1024 ? 2 : 1)));
     const int stages = std::min(kRingStages, kRingBytes / per_sm / stage);
     if (vecs <= 64 || vecs > 2048 || stages < 2) return cudaErrorNotSupported;
-    const int blocks = static_cast<int>(std::min<int64_t>(a.rows, static_cast<int64_t>(num_sms()) * per_sm));
+    // kPhase: rows of one offset in a CTA (one row, or rows a multiple of 8 apart)
+    const int most = kRows == kPhase ? num_sms() * per_sm & ~7 : num_sms() * per_sm;
+    const int blocks = static_cast<int>(std::min<int64_t>(a.rows, most));
     auto run = [&](auto tc, auto kc) -> cudaError_t {
         constexpr int kThreads = decltype(tc)::value, KV = decltype(kc)::value;
         static std::atomic<uint64_t> allowed{0};
-        const cudaError_t e = allow_smem(rms_bwd_ring_kernel<T, kAligned, kThreads, KV>, allowed, kRingBytes);
+        const cudaError_t e = allow_smem(rms_bwd_ring_kernel<T, kRows, kThreads, KV>, allowed, kRingBytes);
         if (e != cudaSuccess) return e;
-        rms_bwd_ring_kernel<T, kAligned, kThreads, KV><<<blocks, kThreads, stages * stage, st>>>(a, stages);
+        rms_bwd_ring_kernel<T, kRows, kThreads, KV><<<blocks, kThreads, stages * stage, st>>>(a, stages);
         const cudaError_t l = cudaGetLastError();
         return l != cudaSuccess ? l : sum_gw<T>(a, blocks, st);
     };
@@ -554,13 +661,16 @@ cudaError_t ring_bwd(const RmsBwdArgs& a, cudaStream_t st) {
     if (vecs <= 256) return run(integral_constant<int, 128>{}, integral_constant<int, 2>{});
     if (vecs <= 512) return run(integral_constant<int, 256>{}, integral_constant<int, 2>{});
     if (vecs <= 1024) return run(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+    if constexpr (kRows == kPhase)
+        if (vecs <= 1152) return run(integral_constant<int, 384>{}, integral_constant<int, 3>{});
     return run(integral_constant<int, 512>{}, integral_constant<int, 4>{});
 }
 
-template <typename T, bool kAligned>
-cudaError_t bwd(const RmsBwdArgs& a, cudaStream_t st) {
+template <typename T, Rows kRows>
+cudaError_t bwd(const RmsBwdArgs& a, bool phase, cudaStream_t st) {
     if (a.rows <= 0) return a.partial ? cudaMemsetAsync(a.gw, 0, a.dim * (a.w_f32 ? sizeof(float) : sizeof(T)), st) : cudaSuccess;
-    const cudaError_t e = ring_bwd<T, kAligned>(a, st);
+    cudaError_t e = phase ? ring_bwd<T, kPhase>(a, st) : cudaErrorNotSupported;
+    if (e == cudaErrorNotSupported) e = ring_bwd<T, kRows>(a, st);
     if (e != cudaErrorNotSupported) return e;
     const int vecs = (a.dim + VecOf<T>::kN - 1) / VecOf<T>::kN;
     auto run = [&](auto kern, int rows_cta, int threads, int per_sm) -> cudaError_t {
@@ -570,9 +680,9 @@ cudaError_t bwd(const RmsBwdArgs& a, cudaStream_t st) {
         const cudaError_t l = cudaGetLastError();
         return l != cudaSuccess ? l : sum_gw<T>(a, blocks, st);
     };
-    if (vecs <= 32) return run(rms_bwd_kernel<T, kAligned, 32, 1>, 8, 256, 3);
-    if (vecs <= 64) return run(rms_bwd_kernel<T, kAligned, 32, 2>, 8, 256, 3);
-    if constexpr (sizeof(T) == 4) return run(rms_bwd_kernel<T, kAligned, 1024, 4>, 1, 1024, 1);
+    if (vecs <= 32) return run(rms_bwd_kernel<T, kRows, 32, 1>, 8, 256, 3);
+    if (vecs <= 64) return run(rms_bwd_kernel<T, kRows, 32, 2>, 8, 256, 3);
+    if constexpr (sizeof(T) == 4) return run(rms_bwd_kernel<T, kRows, 1024, 4>, 1, 1024, 1);
     return cudaErrorInvalidValue;
 }
 
@@ -589,7 +699,9 @@ cudaError_t launch_rms_bwd(Elt et, const RmsBwdArgs& a, cudaStream_t st) {
         constexpr int kN = VecOf<T>::kN;
         const bool whole = a.dim % kN == 0 && aligned(a.h) && a.ldh % kN == 0 && a.ldgy % kN == 0 && aligned(a.gy) &&
                            (!a.gh || (a.ldgh % kN == 0 && aligned(a.gh)));
-        return whole ? bwd<T, true>(a, st) : bwd<T, false>(a, st);
+        const bool phase = (a.ldh - a.dim) % kN == 0 && aligned(a.h) && (a.ldgy - a.dim) % kN == 0 && aligned(a.gy) &&
+                           (!a.gh || ((a.ldgh - a.dim) % kN == 0 && aligned(a.gh)));
+        return whole ? bwd<T, kWhole>(a, false, st) : bwd<T, kAny>(a, phase, st);
     });
 }
 

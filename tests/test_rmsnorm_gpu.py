@@ -184,6 +184,53 @@ def test_quantised_norm(cuda_device, fmt, dtype, rows, dim):
         assert (np.abs(v - val) <= half * step + smallest)[same].all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim", [(5, 3), (40, 333), (33, 1111), (19, 8191)])
+def test_rows_at_different_offsets(cuda_device, dtype, rows, dim):
+    """Inputs whose rows are not equally far past a 16-byte boundary."""
+    x, r, w, gy, gh = _inputs(rows, dim, dtype, dtype, seed=7)
+
+    def shifted(t, k, pad):
+        big = torch.full((rows, dim + pad), float("nan"), dtype=dtype, device=cuda_device)
+        big[:, k:k + dim] = t.to(cuda_device)
+        return big[:, k:k + dim]
+    xd, rd = shifted(x, 1, 5).requires_grad_(), shifted(r, 2, 2).requires_grad_()
+    wd = w.to(cuda_device).requires_grad_()
+    y, h = ops.add_rms_norm(xd, rd, wd, EPS)
+    assert torch.equal(h.detach().cpu(), (x.float() + r.float()).to(dtype))
+    gx, _, gw = torch.autograd.grad([y, h], [xd, rd, wd], [shifted(gy, 3, 4), shifted(gh, 0, 1)])
+    y64, gx64, gw64, mag, gmag = _formulas(h.detach().cpu(), w, gy, gh)
+    u = (dim / 2 + 8) * 2.0 ** -24
+    assert ((y.detach().cpu().double() - y64).abs() <= (u + UNIT[dtype]) * y64.abs() + TINY[dtype]).all()
+    assert ((gx.cpu().double() - gx64).abs() <= (2.5 * dim + 24) * 2.0 ** -24 * mag + UNIT[dtype] * gx64.abs() + TINY[dtype]).all()
+    assert ((gw.cpu().double() - gw64).abs() <= (rows + dim / 2 + 16) * 2.0 ** -24 * gmag + UNIT[dtype] * gw64.abs() + TINY[dtype]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [5, 333, 1111, 4097, 9215])
+def test_a_bad_row_leaves_its_neighbours(cuda_device, dtype, dim):
+    """NaN and infinity in a row that shares 16-byte granules with the rows around it."""
+    x, r, w, gy, gh = (t.to(cuda_device) for t in _inputs(9, dim, dtype, dtype, seed=8))
+    good = [0, 1, 2, 4, 5, 7, 8]
+
+    def results(xx, gg):
+        xs, rs = xx.clone().requires_grad_(), r.clone().requires_grad_()
+        y, h = ops.add_rms_norm(xs, rs, w, EPS)
+        g = torch.autograd.grad([y, h], xs, [gg, gh])[0]
+        with torch.no_grad():
+            t, h8 = ops.rms_norm_quantized(xx, w, residual=r)
+            y1 = ops.rms_norm(xx, w, EPS)
+        return y, h, g, y1, h8, t.dequantize()
+    want = results(x, gy)
+    bad, bad_gy = x.clone(), gy.clone()
+    bad[3], bad[6] = float("nan"), float("inf")
+    bad_gy[3], bad_gy[6] = float("-inf"), float("nan")
+    for a, b in zip(results(bad, bad_gy), want):
+        assert torch.equal(a[good], b[good]) and not a[3].isfinite().all() and not a[6].isfinite().all()
+
+
 def test_norm_cpu_definition():
     x, r, w, gy, gh = _inputs(5, 40, torch.float32, torch.float32)
     xs, rs, ws = (t.clone().requires_grad_() for t in (x, r, w))
