@@ -100,18 +100,33 @@ __global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 4 : 2)
     }
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t amax_bits_of(const uint4& w) {
-    float f[VecOf<T>::kN];
-    unpack16(w, f, T());
+// Largest finite magnitude of kVecs vectors, as bits.  Infinities and NaN have bits above every number's: only where the
+// plain maximum shows one are the elements looked at again one by one.
+template <typename T, int kVecs>
+__device__ __forceinline__ uint32_t finite_amax_bits(const uint4* w) {
+    constexpr int kN = VecOf<T>::kN;
+    constexpr uint32_t kInf = 0x7f800000u;
     uint32_t m = 0;
+    float f[kN];
 #pragma unroll
-    for (int e = 0; e < VecOf<T>::kN; ++e) m = max(m, abs_bits(f[e]));
+    for (int u = 0; u < kVecs; ++u) {
+        unpack16(w[u], f, T());
+#pragma unroll
+        for (int e = 0; e < kN; ++e) m = max(m, abs_bits(f[e]));
+    }
+    if (m < kInf) return m;
+    m = 0;
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+        unpack16(w[u], f, T());
+#pragma unroll
+        for (int e = 0; e < kN; ++e) m = max(m, abs_bits(f[e]) < kInf ? abs_bits(f[e]) : 0u);
+    }
     return m;
 }
 
-// Largest magnitude of each CTA's part of a matrix, as bits (an order that keeps NaN; max does not depend on the order);
-// the pass that reads them takes the largest.  A dense matrix is read as one row.
+// Largest finite magnitude of each CTA's part of a matrix, as bits (max does not depend on the order); the pass that
+// reads them takes the largest.  A dense matrix is read as one row.
 template <typename T>
 __global__ void __launch_bounds__(kAmaxThreads) mx_amax_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t dim,
                                                       uint32_t* __restrict__ amax) {
@@ -131,12 +146,12 @@ __global__ void __launch_bounds__(kAmaxThreads) mx_amax_kernel(const T* __restri
             uint4 w[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) w[u] = reinterpret_cast<const uint4*>(row)[i + u * step];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) m = max(m, amax_bits_of<T>(w[u]));
+            m = max(m, finite_amax_bits<T, 4>(w));
         }
         for (; i < total; i += step) {
             const int64_t left = dim - i * kN;
-            m = max(m, amax_bits_of<T>(load_any(row + i * kN, left < kN ? static_cast<int>(left) : kN)));
+            const uint4 w = load_any(row + i * kN, left < kN ? static_cast<int>(left) : kN);
+            m = max(m, finite_amax_bits<T, 1>(&w));
         }
     }
     m = __reduce_max_sync(0xffffffffu, m);

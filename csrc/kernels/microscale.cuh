@@ -151,12 +151,12 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
     }
 }
 
-// Scale of a whole tensor (nvfp4) from its largest magnitude, times 1 / (6 * 448) rounded to fp32: puts the largest
-// block scale at 448.
-// 2^-100 keeps 1 / (s g) finite; a tensor without a finite maximum keeps g = 1.
+// Scale of a whole tensor (nvfp4) from its largest finite magnitude, times 1 / (6 * 448) rounded to fp32: puts the
+// largest block scale at 448.  An infinity or NaN has its block's scale to itself and does not move the others' grid.
+// 2^-100 keeps 1 / (s g) finite; a tensor with nothing finite but zeros keeps g = 1.
 __device__ __forceinline__ float tensor_scale(uint32_t amax_bits) {
     const float a = __uint_as_float(amax_bits);
-    if (amax_bits == 0 || amax_bits >= 0x7f800000u) return 1.0f;
+    if (amax_bits == 0) return 1.0f;
     return fmaxf(a * (1.0f / 2688.0f), 7.888609052210118e-31f);
 }
 

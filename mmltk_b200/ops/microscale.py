@@ -15,8 +15,8 @@ any sizes are allowed.
 Rounding.  A power-of-two scale is the smallest one with which no element of its block saturates
 (at least 2^-127).  An e4m3 scale is amax / 6 rounded to nearest, on the grid of the tensor scale
 g: elements are x * (1 / (s g)).  Elements round to nearest, ties to even.  A block with an infinity
-or a NaN gets a NaN scale: all its values, and what a product makes of them, are NaN.  For nvfp4,
-g = amax(x) * (1 / 2688, rounded to fp32) unless it is given.
+or a NaN gets a NaN scale: all its values, and what a product makes of them, are NaN; other blocks do not notice.
+For nvfp4, g = (largest finite magnitude of x) * (1 / 2688, rounded to fp32) unless it is given.
 
 Layout.  ``codes`` [rows, pitch]: rows padded to 16 bytes, 4-bit codes two to a byte, the even
 element in the low half (uint8); 8-bit ones float8_e4m3fn.  ``scales`` uint8 [rows / 128, blocks / 4, 32, 4, 4]
@@ -118,9 +118,9 @@ def mx_quantize(x: torch.Tensor, fmt: str, global_scale: Optional[torch.Tensor] 
         raise ValueError("mx_quantize: only nvfp4 has a tensor scale")
     x2 = x.reshape(-1, x.shape[-1]).float()
     if fmt == "nvfp4" and global_scale is None:
-        a = x2.abs().amax() if x2.numel() else x2.new_zeros(())
-        ok = torch.isfinite(a) & (a > 0)
-        global_scale = torch.where(ok, (a * (1.0 / 2688.0)).clamp(min=2.0 ** -100), torch.ones_like(a)).reshape(1)
+        a = x2.abs()
+        a = torch.where(torch.isfinite(a), a, torch.zeros_like(a)).amax() if x2.numel() else x2.new_zeros(())
+        global_scale = torch.where(a > 0, (a * (1.0 / 2688.0)).clamp(min=2.0 ** -100), torch.ones_like(a)).reshape(1)
     codes, scales = quantize_reference(x2, fmt, global_scale)
     return MXTensor(codes, scales, fmt, x.shape, global_scale)
 

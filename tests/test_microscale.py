@@ -33,6 +33,20 @@ def test_tensor_scale_is_found():
         assert ops.mx_quantize(bad, "nvfp4").global_scale.item() == 1.0
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("std", [1e-4, 1.0, 1e4])
+def test_tensor_scale_of_the_finite_values(bad, std):
+    x = torch.randn(6, 80, generator=torch.Generator().manual_seed(11)) * std
+    x[0, :16] = 0
+    want = ops.mx_quantize(x, "nvfp4")
+    y = x.clone()
+    y[0, 3] = bad
+    got = ops.mx_quantize(y, "nvfp4")
+    assert got.global_scale.item() == want.global_scale.item() == tensor_scale(x.numpy())
+    a, b = want.dequantize(torch.float32), got.dequantize(torch.float32)
+    assert torch.isnan(b[0, :16]).all() and torch.equal(a[1:], b[1:]) and torch.equal(a[0, 16:], b[0, 16:])
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_layout_sizes(fmt):
     t = ops.mx_quantize(torch.randn(2, 65, 130), fmt)

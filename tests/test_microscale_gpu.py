@@ -51,6 +51,27 @@ def test_tensor_scale(cuda_device, dtype, rows, dim):
         assert ops.mx_quantize(bad.to(cuda_device), "nvfp4").global_scale.item() == 1.0
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim", [(3, 40), (129, 101), (260, 1000), (1300, 8192)])
+def test_tensor_scale_of_the_finite_values(cuda_device, dtype, rows, dim):
+    """One infinity and one NaN: their blocks are NaN, every other block as without them."""
+    gen = torch.Generator(device=cuda_device).manual_seed(12)
+    x = (torch.randn(rows, dim, device=cuda_device, generator=gen) * 1e-3).to(dtype)
+    x[rows // 2, :16] = 0
+    x[rows - 1, 16:32] = 0
+    bad = x.clone()
+    bad[rows // 2, 5], bad[rows - 1, 16] = float("inf"), float("nan")
+    want, got = ops.mx_quantize(x, "nvfp4"), ops.mx_quantize(bad, "nvfp4")
+    g = (x.float().abs().max().cpu() * (1.0 / 2688.0)).clamp(min=2.0 ** -100)
+    assert got.global_scale.item() == want.global_scale.item() == g.item()
+    a, b = want.dequantize(torch.float32), got.dequantize(torch.float32)
+    a[rows // 2, :16] = a[rows - 1, 16:32] = float("nan")
+    assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.nan_to_num(), b.nan_to_num())
+    wide = torch.full((rows, dim + 3), float("nan"), dtype=dtype, device=cuda_device)      # rows of a view
+    wide[:, 1:1 + dim] = bad
+    assert ops.mx_quantize(wide[:, 1:1 + dim], "nvfp4").global_scale.item() == g.item()
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_quantize_views_and_empty(cuda_device, fmt):
     x = torch.randn(6, 70, 96, generator=torch.Generator().manual_seed(4)).bfloat16().to(cuda_device)
