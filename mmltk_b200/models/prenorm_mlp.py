@@ -36,8 +36,10 @@ class PreNormMlp(nn.Module):
 
     @torch.no_grad()
     def quantize(self, fmt: str = "mxfp8") -> "QuantizedPreNormMlp":
-        return QuantizedPreNormMlp(self.norm_weight.detach(), ops.mx_quantize(self.fc1.weight, fmt), self.fc1.bias,
-                                   ops.mx_quantize(self.fc2.weight, fmt), self.fc2.bias, self.eps)
+        """The serving form of the present parameters: a copy, which later updates of this module do not reach."""
+        copy = lambda t: None if t is None else t.detach().clone()  # noqa: E731
+        return QuantizedPreNormMlp(copy(self.norm_weight), ops.mx_quantize(self.fc1.weight, fmt), copy(self.fc1.bias),
+                                   ops.mx_quantize(self.fc2.weight, fmt), copy(self.fc2.bias), self.eps)
 
 
 class QuantizedPreNormMlp:

@@ -46,6 +46,19 @@ def test_serving_form_cpu(fmt):
         QuantizedPreNormMlp(q.norm_weight, q.w1, q.b1, q.w1, q.b2)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_serving_form_is_a_copy(fmt):
+    m = _block()
+    x, r = torch.randn(9, 96), torch.randn(9, 96)
+    q = m.quantize(fmt)
+    y, h = q(x, r)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.mul_(-3).add_(1)
+    y2, h2 = q(x, r)
+    assert torch.equal(y, y2) and torch.equal(h, h2)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("rows", [1, 20, 300])
