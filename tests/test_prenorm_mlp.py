@@ -47,6 +47,22 @@ def test_serving_form_cpu(fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("size", [1e-5, 1e-2, 1e3])
+def test_serving_form_of_small_and_large_activations(fmt, size):
+    """Inner activations far below and above one keep the format's precision."""
+    m = _block()
+    with torch.no_grad():
+        m.norm_weight.mul_(size)
+        m.fc1.bias.mul_(size)
+        m.fc2.bias.zero_()
+    x, r = torch.randn(9, 96), torch.randn(9, 96)
+    y, _ = m.quantize(fmt)(x, r)
+    y64, _ = _plain(m, x, r)
+    # as above: three operands' roundings in a row, below one operand's worst case
+    assert (y.double() - y64).norm() < (2.0 ** -4 if fmt == "mxfp8" else 0.25) * y64.norm()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_serving_form_is_a_copy(fmt):
     m = _block()
     x, r = torch.randn(9, 96), torch.randn(9, 96)
