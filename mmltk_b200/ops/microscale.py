@@ -131,9 +131,13 @@ def mx_linear(x, weight: MXTensor, bias: Optional[torch.Tensor] = None, *, act: 
     """act(x W^T + bias) with W an ``MXTensor`` [n, k]; fp32 accumulation, one rounding of the output.
 
     ``x``: [..., k] in bf16, fp16 or fp32, quantised to the weight's format in the call, or an ``MXTensor`` of that
-    format.  ``act_scale`` (nvfp4 weight, fp32 [1]): the tensor scale for quantising x (default 1: block
-    maxima from 0.006 to 2688 keep full precision).  ``act``: None, "gelu" (erf) or "relu".  The output is [..., n] in
-    ``out_dtype`` (default: x's dtype, bf16 for an ``MXTensor``) or, with ``out_fmt="mxfp8"``, an ``MXTensor``."""
+    format.  ``act``: None, "gelu" (erf) or "relu".  The output is [..., n] in ``out_dtype`` (default: x's dtype, bf16
+    for an ``MXTensor``) or, with ``out_fmt="mxfp8"``, an ``MXTensor``.
+
+    ``act_scale`` (nvfp4 weight, fp32 [1]): the tensor scale g for quantising x, default 1.  Blocks of x whose maximum
+    lies between 0.094 g and 2688 g keep full precision; below, their e4m3 scales are subnormal and lose bits, blocks
+    under 0.0058 g are zeros (the product is then act(bias)), and values above 2688 g saturate.  For inputs
+    outside that range give amax / 2688, or pass ``mx_quantize(x, "nvfp4")``, which finds it."""
     if act not in _ACTS:
         raise ValueError(f"mx_linear: unknown activation {act!r}")
     if out_fmt not in (None, "mxfp8"):

@@ -63,7 +63,8 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
                        residual: Optional[torch.Tensor] = None, fmt: str = "mxfp8",
                        global_scale: Optional[torch.Tensor] = None) -> Tuple[MXTensor, torch.Tensor]:
     """(quantised RMS norm of h, h), h = x (+ residual): the input of ``mx_linear``, without a 16-bit copy.
-    ``fmt``: "mxfp8", "mxfp4" or "nvfp4" (with its tensor scale, fp32 [1]; default 1).  No gradient."""
+    ``fmt``: "mxfp8", "mxfp4" or "nvfp4" (with its tensor scale, fp32 [1]; default 1: blocks with maxima from 0.094 to
+    2688 keep full precision, see ``mx_linear``).  No gradient."""
     f = format_id(fmt)
     if x.is_cuda:
         codes, scales, h = _kernels().rms_norm_quantized(x, weight, residual, eps, f, global_scale)

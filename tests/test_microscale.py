@@ -47,6 +47,22 @@ def test_tensor_scale_of_the_finite_values(bad, std):
     assert torch.isnan(b[0, :16]).all() and torch.equal(a[1:], b[1:]) and torch.equal(a[0, 16:], b[0, 16:])
 
 
+@pytest.mark.parametrize("g", [1.0, 2.0 ** -20, 3e4])
+def test_range_of_a_tensor_scale(g):
+    """What the products' and norms' documentation says of block maxima on the grid of a given scale."""
+    x = torch.randn(500, 16, generator=torch.Generator().manual_seed(13))
+    x = x / x.abs().amax(1, keepdim=True)
+
+    def worst(top):
+        v = (x * top * g).float()
+        return ((ops.mx_quantize(v, "nvfp4", torch.tensor([g])).dequantize(torch.float32) - v).abs() / (top * g)).max().item()
+    # a normal e4m3 scale is off by 1 / 16 at most, an element by half its largest step: 17 / 16 / 6, and fp32's roundings
+    assert all(worst(top) <= 17 / 96 + 1e-5 for top in (0.094, 0.1, 0.3, 1.0, 40.0, 2688.0))
+    assert worst(0.0175) > 0.25 and worst(0.0058) == 1.0 and worst(4000.0) > 0.32
+    v = x * 1e-6 * g      # the scale that is found fits
+    assert ((ops.mx_quantize(v, "nvfp4").dequantize(torch.float32) - v).abs() <= (17 / 96 + 1e-5) * 1e-6 * g).all()
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_layout_sizes(fmt):
     t = ops.mx_quantize(torch.randn(2, 65, 130), fmt)
