@@ -33,12 +33,12 @@ __global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 4 : 2)
     __shared__ __align__(16) uint8_t tile[kAtoms * kLines * 16];
     __shared__ uint32_t warp_max[kQThreads / 32];
     allow_next();
+    wait_previous();
     // with amax the maximum was found by a pass in ascending order just before: going backwards, this pass
     // finds the end of x still in L2
     const int unit = amax ? units - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x);
     const int ct = unit % col_tiles, line = unit / col_tiles;
     float g = 1.f;
-    if (!amax) wait_previous();
     if constexpr (!Tr::kPow2) {
         if (!amax && g_io) g = *g_io;
     }
@@ -54,7 +54,6 @@ __global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 4 : 2)
     }
     if constexpr (!Tr::kPow2) {
         if (amax) {
-            wait_previous();      // for the maxima; x was complete before that pass let this one start
             uint32_t m = 0;
             for (int i = threadIdx.x; i < parts; i += kQThreads) m = max(m, amax[i]);
             m = __reduce_max_sync(0xffffffffu, m);
@@ -133,8 +132,8 @@ __global__ void __launch_bounds__(kAmaxThreads) mx_amax_kernel(const T* __restri
     constexpr int kN = VecOf<T>::kN;
     __shared__ uint32_t warp_max[kAmaxThreads / 32];
     uint32_t m = 0;
-    wait_previous();      // before the next pass may start: it reads x without waiting for this one
     allow_next();
+    wait_previous();
     // CTAs side by side in a row, then over the rows
     const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
     for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
