@@ -25,6 +25,8 @@ cudaError_t launch_mx_quantize(Elt et, MxFormat f, const void* x, int64_t ld, in
 cudaError_t launch_mx_dequantize(Elt et, MxFormat f, const void* codes, const void* scales, const float* g,
                                  int64_t rows, int64_t dim, void* out, cudaStream_t st);
 
+constexpr int kMxWaitLimit = 1 << 22;
+
 // ---------------------------------------------------------------- RMS norm
 constexpr int kRmsMaxDim = 16384;
 
@@ -58,6 +60,7 @@ struct RmsBwdArgs {
     int* status;          // set when a bounded wait gave up
     int64_t rows, ldgy, ldgh, ldh;
     int dim;
+    int wait_limit;       // tries of a wait for loaded data
     bool w_f32;
 };
 constexpr int rms_partial_pitch(int dim) { return (dim + 7) / 8 * 8; }
@@ -79,6 +82,7 @@ struct MxGemmArgs {
     int* status;
     int64_t x_pitch, w_pitch, y_pitch;   // bytes of a row
     int m, n, k;
+    int wait_limit;           // tries of a wait for loaded data
     Elt out, bias_elt;
     int act;                  // 0 none, 1 GELU, 2 ReLU
     MxFormat fmt;

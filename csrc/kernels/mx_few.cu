@@ -36,7 +36,7 @@ struct FewPlan {
 };
 
 struct __align__(8) FewCtl {
-    uint64_t full[kFewStages], empty[kFewStages], done;
+    uint64_t full[kFewStages], empty[kFewStages], done, drained;
     uint32_t tmem_base;
     int abort;
 };
@@ -72,6 +72,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
             mbar_init(&ctl->empty[s], 1);
         }
         mbar_init(&ctl->done, 1);
+        mbar_init(&ctl->drained, 1);
         ctl->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -177,9 +178,11 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         // the remaining weight stages as the first ones are used up (one warp: MMAs of stage i, then the reload)
         constexpr uint32_t idesc = K::kDesc | (static_cast<uint32_t>(kTok >> 3) << 17) | (128u >> 4 << 24);
         bool ok = true;
+        int loaded = 0;
         for (int i = 0; i < kts; ++i) {
             const int s = i % pl.stages;
-            ok = __all_sync(0xffffffffu, mbar_wait(&ctl->full[s], (i / pl.stages) & 1, &ctl->abort));
+            ok = __all_sync(0xffffffffu, mbar_wait(&ctl->full[s], (i / pl.stages) & 1, &ctl->abort, g.wait_limit));
+            loaded = i + pl.stages;
             if (!ok) break;
             tc_fence_after();
             const uint32_t wa = operand_lo(smem_u32(smem + s * kWTile)), xb = operand_lo(smem_u32(xs + i * kBTile));
@@ -207,9 +210,18 @@ __global__ void __launch_bounds__(kFewThreads, 2)
             }
         }
         if (ok && kts > 0) commit<false>(elected, smem_u32(&ctl->done));
-        if (!ok && elected) {
-            ctl->abort = 1;
-            atomicCAS(g.status, 0, 2);
+        if (!ok) {
+            if (elected) {
+                ctl->abort = 1;
+                atomicCAS(g.status, 0, 2);
+            }
+            // the loads and products that are under way end before anything else happens to their memory
+            commit<false>(elected, smem_u32(&ctl->drained));
+            const unsigned long long deadline = drain_deadline();
+            for (int i = max(0, loaded - pl.stages); i < min(kts, loaded); ++i)
+                mbar_drain(&ctl->full[i % pl.stages], (i / pl.stages) & 1, deadline);
+            mbar_drain(&ctl->drained, 0, deadline);
+            __syncwarp();
         }
     }
     // partial sums to shared memory (over the weight stages, which nothing reads any more): part[t][row]

@@ -89,8 +89,11 @@ struct __align__(8) Ctl {
     uint64_t acc_full[2];
     uint64_t acc_empty[2];
     uint64_t shared_empty[2];     // the columns that both accumulators use have been read
+    uint64_t drained;             // all MMAs of a kernel that gives up
     uint32_t tmem_base;
     int abort;
+    int next_stage;               // where the loading warp stopped, for a drain
+    uint32_t next_phase;
 };
 
 struct Sched {
@@ -347,6 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&ctl->acc_empty[b], kEpiWarps * (kPair ? 2 : 1));
             mbar_init(&ctl->shared_empty[b], 4 * C::kSharers * (kPair ? 2 : 1));
         }
+        mbar_init(&ctl->drained, 1);
         ctl->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -381,7 +385,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             sch.tile(u, mt, nt);
             const int rt = kPair ? 2 * mt + rank : mt;      // this CTA's tile of 128 rows
             for (int kt = kt0; kt < kt0 + kts; ++kt) {
-                if (!__all_sync(0xffffffffu, mbar_wait(&ctl->empty[s], phase, &ctl->abort))) {
+                // (the second look: so that both loading warps of a pair that gives up stop at the same stage)
+                if (!__all_sync(0xffffffffu, mbar_wait(&ctl->empty[s], phase, &ctl->abort)) &&
+                    !__all_sync(0xffffffffu, mbar_try_wait(&ctl->empty[s], phase))) {
                     if (elected) {
                         ctl->abort = 1;
                         atomicCAS(g.status, 0, 1);
@@ -402,6 +408,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     producer_done:
+        if (elected) {
+            ctl->next_stage = s;
+            ctl->next_phase = phase;
+        }
         if constexpr (kSplit) cluster_sync_all();
     } else if (warp == 1) {
         if (rank == 0) {
@@ -433,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 int left = kSplit ? min(g.k - kt0 * K::kElems, kts * K::kElems) : g.k;
                 uint32_t more = 0;
                 for (; ok && left > 0; left -= K::kElems) {
-                    if (!ready) ok = __all_sync(0xffffffffu, mbar_wait(&ctl->full[s], phase, &ctl->abort));
+                    if (!ready) ok = __all_sync(0xffffffffu, mbar_wait(&ctl->full[s], phase, &ctl->abort, g.wait_limit));
                     if (!ok) break;
                     tc_fence_after();
                     // ask for the next stage now and look at the answer after this one's MMAs: a wait costs 170
@@ -475,8 +485,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ready = __all_sync(0xffffffffu, seen);
                 }
                 if (!ok) {
+                    // the MMAs under way end, and their stages are free, before anybody hears of it
+                    commit<kPair>(elected, smem_u32(&ctl->drained));
+                    mbar_drain(&ctl->drained, 0, drain_deadline());
+                    __syncwarp();
                     if (elected) {
                         ctl->abort = 1;
+                        if constexpr (kPair)      // the other CTA's roles wait for this one's barriers
+                            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(smem_u32(&ctl->abort), 1)), "r"(1)
+                                         : "memory");
                         atomicCAS(g.status, 0, 2);
                     }
                     break;
@@ -536,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int c = 0; c < kChunks; ++c) bias_r[c] = bias_at(nt_next * BN + part * kCols + 32 * c + lane);
             }
             const int buf = local & 1;
-            if (!mbar_wait(&ctl->acc_full[buf], (local >> 1) & 1, &ctl->abort)) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&ctl->acc_full[buf], (local >> 1) & 1, &ctl->abort))) {
                 if (lane == 0) atomicCAS(g.status, 0, 3);
                 ctl->abort = 1;
                 if constexpr (kSplit) cluster_sync_all();
@@ -653,6 +670,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
+    if (warp == 0 && rank == 0 && ctl->abort) {
+        // loads that nobody waited for (a pair's count on the even CTA's barriers): the last of each stage, which is of
+        // this turn of the ring below next_stage and of the one before from there on
+        const unsigned long long deadline = drain_deadline();
+        for (int i = 0; i < kStages; ++i)
+            mbar_drain(&ctl->full[i], i < ctl->next_stage ? ctl->next_phase ^ 1 : ctl->next_phase, deadline);
+        __syncwarp();
+    }
     // no CTA leaves while the pair's MMAs, or the cluster's sums, may still read its shared memory
     if constexpr (kPair || kSplit) cluster_sync_all();
     if (warp == 0) {

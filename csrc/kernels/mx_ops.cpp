@@ -4,6 +4,7 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <atomic>
 #include <limits>
 #include <mutex>
 #include <vector>
@@ -100,6 +101,13 @@ int* mx_status_word(const torch::Device& dev) {
     auto& t = words.at(dev.index());
     if (!t.defined()) t = torch::zeros({1}, torch::TensorOptions().dtype(torch::kInt32).device(dev));
     return t.data_ptr<int>();
+}
+
+// Tries that a wait for loaded data makes before the kernel gives up; 0: none (tests of the status word).
+std::atomic<int> wait_limit{kMxWaitLimit};
+int64_t mx_wait_limit(int64_t tries) {
+    TORCH_CHECK(tries >= 0 && tries <= kMxWaitLimit, "mx_wait_limit: 0 to ", kMxWaitLimit, " tries");
+    return wait_limit.exchange(static_cast<int>(tries));
 }
 
 // Non-zero when a kernel on this device gave up a bounded wait (products: 1 loads, 2 MMA, 3 epilogue; 4 norm
@@ -245,6 +253,7 @@ std::pair<torch::Tensor, torch::Tensor> norm_backward(const torch::Tensor& gy, c
     a.w_f32 = w.scalar_type() == torch::kFloat32 && h.scalar_type() != torch::kFloat32;
     a.rstd = rstd.data_ptr<float>();
     a.status = mx_status_word(h.device());
+    a.wait_limit = wait_limit.load(std::memory_order_relaxed);
     auto gx = fresh(h.sizes(), h.scalar_type(), h);
     a.gx = gx.data_ptr();
     torch::Tensor gw;
@@ -375,6 +384,7 @@ std::vector<torch::Tensor> mx_linear(OptTensor x, OptTensor x_codes, OptTensor x
     }
     if (rows && n) {
         a.status = mx_status_word(w_codes.device());
+        a.wait_limit = wait_limit.load(std::memory_order_relaxed);
         if (mx_few_fits(f, a.m, a.n, a.k, !xr.defined())) {
             MxFewArgs few{};
             if (xr.defined()) {
@@ -420,6 +430,7 @@ void register_mx_ops(pybind11::module& m) {
           py::arg("fmt"), py::arg("g") = py::none());
     m.def("mx_linear", &mx_linear);
     m.def("mx_status", &mx_status);
+    m.def("mx_wait_limit", &mx_wait_limit);
 }
 
 }  // namespace mmltk

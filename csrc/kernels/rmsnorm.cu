@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
         const int s = j % stages;
         const int64_t r = first + j * step;
         const float rstd = a.rstd[r];
-        const bool here = tc::mbar_wait(&full[s], (j / stages) & 1, &abort);
+        const bool here = tc::mbar_wait(&full[s], (j / stages) & 1, &abort, a.wait_limit);
         const T* in[3];
 #pragma unroll
         for (int i = 0; i < 3; ++i)
@@ -495,7 +495,13 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
             atomicCAS(a.status, 0, 4);
         }
         sum = group_sum<kThreads>(sum, red[j & 1]);
-        if (abort) break;                        // (seen by all after the barrier in group_sum)
+        if (abort) {                             // (seen by all after the barrier in group_sum)
+            if (t == 0) {
+                const unsigned long long deadline = tc::drain_deadline();
+                for (int i = j; i < min(count, j + stages - 1); ++i) tc::mbar_drain(&full[i % stages], (i / stages) & 1, deadline);
+            }
+            break;
+        }
         if (t == 0 && j + stages - 1 < count) load(j + stages - 1);
         const float c = sum * inv_dim * rstd * rstd * rstd;
 #pragma unroll

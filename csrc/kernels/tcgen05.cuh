@@ -42,12 +42,25 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 // Bounded wait; false on timeout or when another role has aborted.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const volatile int* abort) {
-    for (long long i = 0; i < kWaitLimit; ++i) {
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const volatile int* abort,
+                                          long long limit = kWaitLimit) {
+    for (long long i = 0; i < limit; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((i & 255) == 255 && *abort) return false;
     }
     return false;
+}
+// For a kernel that gives up: what is still on its way to this CTA's memory has to land before the CTA leaves.  The waits
+// of one drain share a deadline, a second from drain_deadline.
+__device__ __forceinline__ unsigned long long drain_clock() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ unsigned long long drain_deadline() { return drain_clock() + 1000000000ull; }
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity, unsigned long long deadline) {
+    while (!mbar_try_wait(bar, parity) && drain_clock() < deadline) {
+    }
 }
 __device__ __forceinline__ void tma_load_2d(const CUtensorMap* map, uint64_t* bar, void* dst, int c0, int c1) {
     asm volatile(

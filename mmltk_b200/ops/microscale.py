@@ -53,6 +53,7 @@ _BLOCK = {"mxfp4": 32, "nvfp4": 16, "mxfp8": 32}
 _BITS = {"mxfp4": 4, "nvfp4": 4, "mxfp8": 8}
 _ACTS = {None: 0, "none": 0, "gelu": 1, "relu": 2}
 _E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+WAIT_LIMIT = 1 << 22      # tries of a kernel's bounded wait (``kernels().mx_wait_limit``)
 _OUT_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
