@@ -253,6 +253,12 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     }
     tc_fence_before();
     __syncthreads();
+    // tensor memory is given back before this CTA waits for its cluster: a CTA that held some could wait for one that
+    // cannot get any, behind a kernel of another stream that in turn waits for this CTA's
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(128));
+    }
     cluster_sync_all();
 
     // outputs: 128 rows of w x m tokens, dealt to the cluster's CTAs; a warp has 32 neighbours of one token
@@ -306,10 +312,6 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         for (int t = g.m + threadIdx.x; t < 128; t += kFewThreads)
             *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(g.scales) + scale_offset(t, 4 * nt, ykt)) = 0;
     cluster_sync_all();      // nobody's shared memory goes while another CTA reads it
-    if (warp == 0) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(128));
-    }
 }
 
 // Slices and shared memory of an m x n x k product; splits = 0: does not fit (x's slice is held whole).
