@@ -2,6 +2,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <atomic>
@@ -94,13 +95,29 @@ void no_grad_here(const torch::Tensor& t, const char* what) {
                 ": has no gradient (a serving operator); call it under torch.no_grad() or on detached tensors");
 }
 
+// The current device's status word: allocated and cleared before the first call that takes it returns, on a stream of its
+// own, so that a first call under graph capture leaves no clear in the graph (its replays would erase what they record).
 int* mx_status_word(const torch::Device& dev) {
     static std::mutex mu;
-    static std::vector<torch::Tensor> words(64);
+    static std::vector<int*> words(64);
     std::lock_guard<std::mutex> lk(mu);
-    auto& t = words.at(dev.index());
-    if (!t.defined()) t = torch::zeros({1}, torch::TensorOptions().dtype(torch::kInt32).device(dev));
-    return t.data_ptr<int>();
+    int*& word = words.at(dev.index());
+    if (!word) {
+        c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+        int* p = nullptr;
+        cudaStream_t own = nullptr;
+        check_cuda(cudaMalloc(reinterpret_cast<void**>(&p), sizeof(int)), "mx_status");
+        cudaError_t e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+        if (e == cudaSuccess) {
+            e = cudaMemsetAsync(p, 0, sizeof(int), own);
+            if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+            cudaStreamDestroy(own);
+        }
+        if (e != cudaSuccess) cudaFree(p);
+        check_cuda(e, "mx_status");
+        word = p;
+    }
+    return word;
 }
 
 // Tries that a wait for loaded data makes before the kernel gives up; 0: none (tests of the status word).
@@ -111,15 +128,16 @@ int64_t mx_wait_limit(int64_t tries) {
 }
 
 // Non-zero when a kernel on this device gave up a bounded wait (products: 1 loads, 2 MMA, 3 epilogue; 4 norm
-// backward); clears it.
+// backward); waits for all work on the device, and clears it.
 int64_t mx_status(int64_t device) {
     const torch::Device dev(torch::kCUDA, static_cast<c10::DeviceIndex>(device));
     at::cuda::CUDAGuard guard(dev);
     int* w = mx_status_word(dev);
+    const int zero = 0;
     int v = 0;
-    check_cuda(cudaMemcpyAsync(&v, w, sizeof(v), cudaMemcpyDeviceToHost, cur_stream()), "mx_status");
-    check_cuda(cudaStreamSynchronize(cur_stream()), "mx_status");
-    if (v) check_cuda(cudaMemsetAsync(w, 0, sizeof(int), cur_stream()), "mx_status");
+    check_cuda(cudaDeviceSynchronize(), "mx_status");
+    check_cuda(cudaMemcpy(&v, w, sizeof(v), cudaMemcpyDeviceToHost), "mx_status");
+    if (v) check_cuda(cudaMemcpy(w, &zero, sizeof(v), cudaMemcpyHostToDevice), "mx_status");
     return v;
 }
 

@@ -188,7 +188,9 @@ def mx_linear(x, weight: MXTensor, bias: Optional[torch.Tensor] = None, *, act: 
 
 
 def mx_status(device=None) -> int:
-    """Non-zero when a product on ``device`` gave up a bounded wait since the last call (its output is then invalid)."""
+    """Non-zero when a product, or a norm's backward, on ``device`` gave up a bounded wait since the last call: outputs
+    since then may be invalid.  Nothing else reports it, so a program asks where it waits for results anyway (the call
+    waits for all streams of the device; not under graph capture)."""
     dev = torch.device("cuda" if device is None else device)
     return _kernels().mx_status(torch.cuda.current_device() if dev.index is None else dev.index)
 

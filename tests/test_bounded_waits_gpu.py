@@ -1,4 +1,8 @@
 """A bounded wait that runs out: the call returns, the status word says so, and the GPU goes on."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -63,6 +67,45 @@ def test_a_wait_that_runs_out(cuda_device, name, no_wait):
         assert ops.mx_status(cuda_device) == 0    # the read cleared it
         k.mx_wait_limit(ops.microscale.WAIT_LIMIT)
         assert torch.equal(_bits(run()), want) and ops.mx_status(cuda_device) == 0
+
+
+FIRST_CALL_CAPTURED = """
+import torch
+from mmltk_b200 import ops
+from mmltk_b200.ops import kernels
+x = torch.randn(64, 700, device="cuda").bfloat16()
+w = ops.mx_quantize(torch.randn(200, 700, device="cuda"), "mxfp8")
+good, bad = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+with torch.cuda.graph(good):                 # the process's first product
+    a = ops.mx_linear(x, w)
+was = kernels().mx_wait_limit(0)
+with torch.cuda.graph(bad):
+    b = ops.mx_linear(x, w)
+kernels().mx_wait_limit(was)
+assert ops.mx_status() == 0                  # nothing has run
+bad.replay()
+good.replay()                                # does not erase what the other one recorded
+assert ops.mx_status() != 0 and ops.mx_status() == 0
+want = ops.mx_linear(x, w)
+good.replay()
+assert torch.equal(a, want) and ops.mx_status() == 0
+side = torch.cuda.Stream()
+side.wait_stream(torch.cuda.current_stream())
+kernels().mx_wait_limit(0)
+with torch.cuda.stream(side):
+    for _ in range(20):
+        big = torch.randn(4096, 4096, device="cuda") @ torch.randn(4096, 4096, device="cuda")
+    ops.mx_linear(x, w)
+kernels().mx_wait_limit(was)
+assert ops.mx_status() != 0                  # of another stream, still running
+print("checked")
+"""
+
+
+def test_status_of_a_captured_first_call_and_of_other_streams():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], cwd=root, capture_output=True, text=True, timeout=200)
+    assert r.returncode == 0 and r.stdout.strip() == "checked", r.stdout + r.stderr
 
 
 def test_wait_limit_is_checked():
