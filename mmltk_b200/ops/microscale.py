@@ -95,11 +95,37 @@ class MXTensor:
             y = _kernels().mx_dequantize(self.codes, self.scales, self.global_scale, _FORMATS[self.fmt], self.rows,
                                          self.shape[-1], dtype)
         else:
+            if dtype not in _OUT_DTYPES:
+                raise TypeError(f"mx_dequantize: bf16, fp16 or fp32 expected, got {dtype}")
+            _check_coded(self, "mx_dequantize")
             y = dequantize_reference(self).to(dtype)
         return y if len(self.shape) == 2 else y.view(self.shape)
 
     def __repr__(self) -> str:
         return f"MXTensor({self.fmt}, shape={self.shape}, device={self.device})"
+
+
+# What the kernels' wrappers refuse, for CPU tensors.
+def _check_coded(t: MXTensor, what: str) -> None:
+    rows, dim, bits = t.rows, t.shape[-1], _BITS[t.fmt]
+    pitch, tiles = -(-dim * bits // 128) * 16, -(-dim // (4 * _BLOCK[t.fmt]))
+    if (t.codes.dtype != (torch.float8_e4m3fn if bits == 8 else torch.uint8) or tuple(t.codes.shape) != (rows, pitch)
+            or not t.codes.is_contiguous()):
+        raise ValueError(f"{what}: codes of {t} must be contiguous [{rows}, {pitch}]")
+    if (t.scales.dtype != torch.uint8 or t.scales.device != t.codes.device or not t.scales.is_contiguous()
+            or t.scales.numel() != -(-rows // 128) * tiles * 512):
+        raise ValueError(f"{what}: scales of {t} must be contiguous uint8 [{-(-rows // 128)}, {tiles}, 32, 4, 4]")
+
+
+def _check_scalar(g: Optional[torch.Tensor], like: torch.Tensor, what: str) -> None:
+    if g is not None and (g.dtype != torch.float32 or g.numel() != 1 or g.device != like.device):
+        raise ValueError(f"{what}: the tensor scale is one fp32 value on the same device")
+
+
+def _no_grad_here(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what}: has no gradient (a serving operator); call it under torch.no_grad() or on "
+                           "detached tensors")
 
 
 def mx_quantize(x: torch.Tensor, fmt: str, global_scale: Optional[torch.Tensor] = None) -> MXTensor:
@@ -113,10 +139,10 @@ def mx_quantize(x: torch.Tensor, fmt: str, global_scale: Optional[torch.Tensor] 
         raise ValueError("mx_quantize: needs a last dimension of at least one element")
     if x.dtype not in _OUT_DTYPES:
         raise TypeError(f"mx_quantize: bf16, fp16 or fp32 expected, got {x.dtype}")
-    if torch.is_grad_enabled() and x.requires_grad:
-        raise RuntimeError("mx_quantize: has no gradient (a serving operator)")
+    _no_grad_here("mx_quantize", x)
     if global_scale is not None and fmt != "nvfp4":
         raise ValueError("mx_quantize: only nvfp4 has a tensor scale")
+    _check_scalar(global_scale, x, "mx_quantize")
     x2 = x.reshape(-1, x.shape[-1]).float()
     if fmt == "nvfp4" and global_scale is None:
         a = x2.abs()
@@ -173,7 +199,20 @@ def mx_linear(x, weight: MXTensor, bias: Optional[torch.Tensor] = None, *, act: 
         if out_fmt is not None:
             return MXTensor(out[0], out[1], out_fmt, shape)
         return out[0] if len(shape) == 2 else out[0].view(shape)
-    if not quantised:
+    _check_coded(weight, "mx_linear: weight")
+    _check_scalar(weight.global_scale, weight.codes, "mx_linear: weight")
+    if x.device != weight.device:
+        raise ValueError("mx_linear: input and weight on different devices")
+    if bias is not None:
+        if bias.device != weight.device or bias.shape != (n,):
+            raise ValueError(f"mx_linear: bias must be [{n}] on the weight's device")
+        if bias.dtype not in _OUT_DTYPES:
+            raise TypeError(f"mx_linear: bias in bf16, fp16 or fp32, got {bias.dtype}")
+        _no_grad_here("mx_linear", bias)
+    if quantised:
+        _check_coded(x, "mx_linear: input")
+        _check_scalar(x.global_scale, x.codes, "mx_linear: input")
+    else:
         if x.shape[-1] != k:
             raise ValueError(f"mx_linear: input [..., {k}] expected, got {tuple(x.shape)}")
         one = torch.ones(1) if fmt == "nvfp4" else None

@@ -16,20 +16,25 @@ from typing import Optional, Tuple
 
 import torch
 
-from .microscale import MXTensor, _kernels, format_id, quantize_reference
+from .microscale import MXTensor, _check_scalar, _kernels, _no_grad_here, format_id, quantize_reference
 
 __all__ = ["rms_norm", "add_rms_norm", "rms_norm_quantized"]
 
 
-def _check(x, weight, residual):
+MAX_DIM = 16384      # elements of a row
+
+
+def _check(x, weight, residual):      # what the kernels' wrappers refuse, for CPU tensors
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("rms_norm: needs a last dimension of at least one element")
-    if not x.is_floating_point() or x.dtype == torch.float64:
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise TypeError(f"rms_norm: bf16, fp16 or fp32 expected, got {x.dtype}")
-    if weight.shape != x.shape[-1:]:
-        raise ValueError(f"rms_norm: weight must be [{x.shape[-1]}], got {tuple(weight.shape)}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError("rms_norm: residual must match the input's shape and dtype")
+    if x.shape[-1] > MAX_DIM:
+        raise ValueError(f"rms_norm: rows of at most {MAX_DIM} elements")
+    if weight.device != x.device or weight.shape != x.shape[-1:] or weight.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"rms_norm: weight must be [{x.shape[-1]}] of the input's dtype or fp32, on its device")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError("rms_norm: residual must match the input's shape, dtype and device")
 
 
 def _reference(x, weight, residual, eps):
@@ -70,10 +75,10 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
         codes, scales, h = _kernels().rms_norm_quantized(x, weight, residual, eps, f, global_scale)
         return MXTensor(codes, scales, fmt, x.shape, global_scale), x if residual is None else h
     _check(x, weight, residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
-        raise RuntimeError("rms_norm_quantized: has no gradient (a serving operator)")
+    _no_grad_here("rms_norm_quantized", x, weight, residual)
     if global_scale is not None and fmt != "nvfp4":
         raise ValueError("rms_norm_quantized: only nvfp4 has a tensor scale")
+    _check_scalar(global_scale, x, "rms_norm_quantized")
     y, h = _reference(x, weight, residual, eps)
     codes, scales = quantize_reference(y.reshape(-1, x.shape[-1]), fmt, global_scale)
     return MXTensor(codes, scales, fmt, x.shape, global_scale), h

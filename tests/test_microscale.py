@@ -158,6 +158,61 @@ def test_refusals_gpu(cuda_device):
             call()
 
 
+def _more_refusals(dev):
+    """What the kernels' wrappers refuse, on any device."""
+    x, w = torch.randn(4, 64, device=dev), ops.mx_quantize(torch.randn(8, 64, device=dev), "mxfp4")
+    wn = ops.mx_quantize(torch.randn(8, 64, device=dev), "nvfp4")
+    ones = torch.ones(64, device=dev)
+    two = torch.ones(2, device=dev)
+    calls = [
+        lambda: ops.mx_linear(x, w, torch.ones(1, device=dev)),
+        lambda: ops.mx_linear(x, w, torch.ones(9, device=dev)),
+        lambda: ops.mx_linear(x, w, torch.ones(4, 8, device=dev)),
+        lambda: ops.mx_linear(x, w, torch.ones(8, device=dev).double()),
+        lambda: ops.mx_linear(x, w, torch.ones(8, device=dev, requires_grad=True)),
+        lambda: ops.mx_linear(x.clone().requires_grad_(), w),
+        lambda: ops.mx_linear(x, wn, act_scale=two),
+        lambda: ops.mx_linear(x, wn, act_scale=two[:1].double()),
+        lambda: ops.mx_linear(x, MXTensor(w.codes[:4], w.scales, "mxfp4", (8, 64))),
+        lambda: ops.mx_linear(x, MXTensor(w.codes, w.scales[..., :2], "mxfp4", (8, 64))),
+        lambda: ops.mx_linear(x, MXTensor(w.codes.float(), w.scales, "mxfp4", (8, 64))),
+        lambda: ops.mx_linear(x, MXTensor(w.codes, w.scales.int(), "mxfp4", (8, 64))),
+        lambda: ops.mx_linear(x, MXTensor(wn.codes, wn.scales, "nvfp4", (8, 64), two)),
+        lambda: ops.mx_linear(MXTensor(w.codes[:4], w.scales, "mxfp4", (8, 64)), w),
+        lambda: MXTensor(w.codes, w.scales, "mxfp4", (9, 64)).dequantize(),
+        lambda: w.dequantize(torch.float64),
+        lambda: ops.mx_quantize(x, "nvfp4", two),
+        lambda: ops.mx_quantize(x, "nvfp4", two[:1].double()),
+        lambda: ops.rms_norm(x, ones.double()),
+        lambda: ops.rms_norm(x, ones.bfloat16()),
+        lambda: ops.rms_norm(x, ones.long()),
+        lambda: ops.rms_norm(x.to(torch.float8_e4m3fn), ones),
+        lambda: ops.rms_norm(torch.zeros(2, 16385, device=dev), torch.ones(16385, device=dev)),
+        lambda: ops.rms_norm_quantized(x, ones, fmt="nvfp4", global_scale=two),
+        lambda: ops.rms_norm_quantized(x, ones.clone().requires_grad_()),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            call()
+            pytest.fail(f"call {i} was accepted")
+    with torch.no_grad():
+        ops.mx_linear(x, w, torch.ones(8, device=dev, requires_grad=True))
+
+
+def test_more_refusals_cpu():
+    _more_refusals("cpu")
+
+
+@pytest.mark.gpu
+def test_more_refusals_gpu(cuda_device):
+    _more_refusals(cuda_device)
+    x, w = torch.randn(4, 64), ops.mx_quantize(torch.randn(8, 64), "mxfp4")
+    for call in (lambda: ops.mx_linear(x.to(cuda_device), w), lambda: ops.mx_linear(x, w, torch.ones(8, device=cuda_device)),
+                 lambda: ops.rms_norm(x, torch.ones(64, device=cuda_device))):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            call()
+
+
 def test_an_error_message_with_a_number_reaches_python():
     # formatted by the extension itself: needs the process's libstdc++ (it crashed on a private copy)
     c = torch.zeros(2, 16, dtype=torch.uint8)
