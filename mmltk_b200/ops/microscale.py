@@ -71,6 +71,8 @@ class MXTensor:
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str, shape: Sequence[int],
                  global_scale: Optional[torch.Tensor] = None):
         format_id(fmt)
+        if global_scale is not None and fmt != "nvfp4":
+            raise ValueError(f"MXTensor: only nvfp4 has a tensor scale, not {fmt}")
         self.codes, self.scales, self.fmt, self.shape, self.global_scale = codes, scales, fmt, tuple(shape), global_scale
 
     @property

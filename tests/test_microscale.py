@@ -158,6 +158,14 @@ def test_refusals_gpu(cuda_device):
             call()
 
 
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+def test_a_tensor_scale_belongs_to_nvfp4(fmt):
+    # (the plain definition and the product applied one to the other formats too, the kernel that reads values back did not)
+    t = ops.mx_quantize(torch.randn(3, 40), fmt)
+    with pytest.raises(ValueError, match="only nvfp4"):
+        MXTensor(t.codes, t.scales, fmt, t.shape, torch.full((1,), 2.0))
+
+
 def _more_refusals(dev):
     """What the kernels' wrappers refuse, on any device."""
     x, w = torch.randn(4, 64, device=dev), ops.mx_quantize(torch.randn(8, 64, device=dev), "mxfp4")
