@@ -38,16 +38,6 @@ from ._ext import kernels
 __all__ = ["MXTensor", "mx_quantize", "mx_linear", "mx_status", "format_id", "quantize_reference",
            "dequantize_reference"]
 
-_ext = []
-
-
-def _kernels():
-    """The kernel extension, looked up once: the lookup reads the environment, a tenth of a small call's time."""
-    if not _ext:
-        _ext.append(kernels())
-    return _ext[0]
-
-
 _FORMATS = {"mxfp4": 0, "nvfp4": 1, "mxfp8": 2}
 _BLOCK = {"mxfp4": 32, "nvfp4": 16, "mxfp8": 32}
 _BITS = {"mxfp4": 4, "nvfp4": 4, "mxfp8": 8}
@@ -94,7 +84,7 @@ class MXTensor:
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values, rounded once to ``dtype`` (bf16, fp16 or fp32)."""
         if self.codes.is_cuda:
-            y = _kernels().mx_dequantize(self.codes, self.scales, self.global_scale, _FORMATS[self.fmt], self.rows,
+            y = kernels().mx_dequantize(self.codes, self.scales, self.global_scale, _FORMATS[self.fmt], self.rows,
                                          self.shape[-1], dtype)
         else:
             if dtype not in _OUT_DTYPES:
@@ -135,7 +125,7 @@ def mx_quantize(x: torch.Tensor, fmt: str, global_scale: Optional[torch.Tensor] 
     tensor scale to use; by default it is found from x (one more pass over it)."""
     f = format_id(fmt)
     if x.is_cuda:
-        codes, scales, g = _kernels().mx_quantize(x, f, global_scale)
+        codes, scales, g = kernels().mx_quantize(x, f, global_scale)
         return MXTensor(codes, scales, fmt, x.shape, g)
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("mx_quantize: needs a last dimension of at least one element")
@@ -192,11 +182,11 @@ def mx_linear(x, weight: MXTensor, bias: Optional[torch.Tensor] = None, *, act: 
     shape = (*x.shape[:-1], n)
     if weight.codes.is_cuda:
         if quantised:
-            out = _kernels().mx_linear(None, x.codes, x.scales, x.global_scale, x.rows, weight.codes, weight.scales,
+            out = kernels().mx_linear(None, x.codes, x.scales, x.global_scale, x.rows, weight.codes, weight.scales,
                                        weight.global_scale, _FORMATS[fmt], n, k, bias, _ACTS[act], out_dtype,
                                        out_fmt is not None)
         else:
-            out = _kernels().mx_linear(x, None, None, act_scale, 0, weight.codes, weight.scales, weight.global_scale,
+            out = kernels().mx_linear(x, None, None, act_scale, 0, weight.codes, weight.scales, weight.global_scale,
                                        _FORMATS[fmt], n, k, bias, _ACTS[act], out_dtype, out_fmt is not None)
         if out_fmt is not None:
             return MXTensor(out[0], out[1], out_fmt, shape)
@@ -233,7 +223,7 @@ def mx_status(device=None) -> int:
     since then may be invalid.  Nothing else reports it, so a program asks where it waits for results anyway (the call
     waits for all streams of the device; not under graph capture)."""
     dev = torch.device("cuda" if device is None else device)
-    return _kernels().mx_status(torch.cuda.current_device() if dev.index is None else dev.index)
+    return kernels().mx_status(torch.cuda.current_device() if dev.index is None else dev.index)
 
 
 # ---------------------------------------------------------------- the plain definition

@@ -16,7 +16,8 @@ from typing import Optional, Tuple
 
 import torch
 
-from .microscale import MXTensor, _check_scalar, _kernels, _no_grad_here, format_id, quantize_reference
+from ._ext import kernels
+from .microscale import MXTensor, _check_scalar, _no_grad_here, format_id, quantize_reference
 
 __all__ = ["rms_norm", "add_rms_norm", "rms_norm_quantized"]
 
@@ -47,7 +48,7 @@ def _reference(x, weight, residual, eps):
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
     """RMS norm over the last dimension, in x's dtype; differentiable."""
     if x.is_cuda:
-        return _kernels().rms_norm(x, weight, None, eps)[0]
+        return kernels().rms_norm(x, weight, None, eps)[0]
     _check(x, weight, None)
     return _reference(x, weight, None, eps)[0].to(x.dtype)
 
@@ -57,7 +58,7 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
     """(RMS norm of h, h) with h = x + residual: the branch's output joins the residual stream and is normalised
     for the next branch in one pass.  The norm reads h as it is stored (rounded to x's dtype); differentiable."""
     if x.is_cuda:
-        y, h = _kernels().rms_norm(x, weight, residual, eps)
+        y, h = kernels().rms_norm(x, weight, residual, eps)
         return y, h
     _check(x, weight, residual)
     y, h = _reference(x, weight, residual, eps)
@@ -72,7 +73,7 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     2688 keep full precision, see ``mx_linear``).  No gradient."""
     f = format_id(fmt)
     if x.is_cuda:
-        codes, scales, h = _kernels().rms_norm_quantized(x, weight, residual, eps, f, global_scale)
+        codes, scales, h = kernels().rms_norm_quantized(x, weight, residual, eps, f, global_scale)
         return MXTensor(codes, scales, fmt, x.shape, global_scale), x if residual is None else h
     _check(x, weight, residual)
     _no_grad_here("rms_norm_quantized", x, weight, residual)

@@ -221,6 +221,36 @@ def test_more_refusals_gpu(cuda_device):
             call()
 
 
+def test_debug_switch_is_looked_up_at_every_call(monkeypatch):
+    from mmltk_b200.ops import _ext
+
+    class Fake:
+        def __init__(self, name):
+            self.name = name
+
+        def __getattr__(self, op):
+            raise LookupError(f"{self.name}.{op}")
+
+    class OnGpu:      # stands for a CUDA tensor, as far as the call looks before it reaches the extension
+        is_cuda, shape, dtype = True, (1, 64), torch.float32
+
+        def __getattr__(self, name):
+            raise AssertionError(name)
+    monkeypatch.setattr(_ext, "_load", lambda name: (Fake(name), None))
+    x = OnGpu()
+    calls = {"mx_quantize": lambda: ops.mx_quantize(x, "mxfp4"), "rms_norm": lambda: ops.rms_norm(x, x),
+             "rms_norm_quantized": lambda: ops.rms_norm_quantized(x, x), "mx_status": lambda: ops.mx_status(torch.device("cuda", 0))}
+    for value, name in (("0", "_kernels"), ("1", "_kernels_dbg"), (None, "_kernels"), ("1", "_kernels_dbg")):
+        if value is None:
+            monkeypatch.delenv("MMLTK_DEBUG_BOUNDS", raising=False)
+        else:
+            monkeypatch.setenv("MMLTK_DEBUG_BOUNDS", value)
+        assert _ext.kernel_module_name() == name
+        for op, call in calls.items():
+            with pytest.raises(LookupError, match=f"^{name}.{op}$"):
+                call()
+
+
 def test_an_error_message_with_a_number_reaches_python():
     # formatted by the extension itself: needs the process's libstdc++ (it crashed on a private copy)
     c = torch.zeros(2, 16, dtype=torch.uint8)
