@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     cluster_sync_all();
 
     // outputs: 128 rows of w x m tokens, dealt to the cluster's CTAs; a warp has 32 neighbours of one token
-    const float alpha = (g.x_g ? *g.x_g : 1.f) * (g.w_g ? *g.w_g : 1.f);
+    const Alpha alpha = F == MxFormat::kNvFp4 ? product_scale(g.x_g, g.w_g) : Alpha{1.f, 1.f};
     const uint32_t part_addr = smem_u32(part);
     uint32_t peers[kFewSplits];
 #pragma unroll
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
             float v = p[o][0];
 #pragma unroll
             for (int s = 1; s < kFewSplits; ++s) v += p[o][s];
-            v = fmaf(v, alpha, bias);
+            v = fmaf(v * alpha.pre, alpha.rest, bias);
             if (g.act == 1) v = gelu_fwd(v);
             else if (g.act == 2) v = v < 0.f ? 0.f : v;    // (keeps a NaN)
             if (g.codes) {

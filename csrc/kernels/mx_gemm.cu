@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         unsigned char* buf_s = staging + (warp - 2) * C::kStaging;
         constexpr int kBox = C::kBox, kRow = C::kRow, kPieces = 32 * kSize / 16;
         float* bias_w = bias_s + (warp - 2) * kCols;
-        const float alpha = (g.x_g ? *g.x_g : 1.f) * (g.w_g ? *g.w_g : 1.f);
+        const Alpha alpha = F == MxFormat::kNvFp4 ? product_scale(g.x_g, g.w_g) : Alpha{1.f, 1.f};
         const int ykt = kQuantOut ? static_cast<int>(mx_scale_tiles(MxFormat::kMxFp8, g.n)) : 0;
         auto bias_at = [&](int col) {
             if (!g.bias || col >= g.n) return 0.f;
@@ -622,8 +622,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sum[j]);
                 }
                 if (col >= g.n || row0 >= g.m) continue;       // warp-uniform
+                if (F == MxFormat::kNvFp4 && alpha.pre != 1.f) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha.pre);
+                }
                 f2 x[16];
-                const f2 alpha2 = pack2(alpha, alpha);
+                const f2 alpha2 = pack2(alpha.rest, alpha.rest);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const ulonglong2 b = reinterpret_cast<const ulonglong2*>(bias_w + 32 * c)[j];

@@ -146,6 +146,26 @@ def test_linear(cuda_device, fmt, m, n, k, dtype, act):
     assert ops.mx_status(cuda_device) == 0
 
 
+@pytest.mark.parametrize("sx,sw", [(1e30, 1e20), (1e-25, 1e-10), (1e-18, 1e-18), (1e-6, 1e-27), (1e30, 1e-30)])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 64), (40, 300, 200), (70, 200, 6200), (2500, 1300, 200)])
+def test_tensor_scales_far_apart_from_one(cuda_device, sx, sw, m, n, k):
+    """Two scales whose product is no normal fp32 number, but the product of a sum and both is."""
+    x, w, _ = _operands(m, n, k, "nvfp4", torch.float32, seed=15)
+    x, w = x * sx, w * sw
+    x[1] = 0
+    w[5] = w[5] * 2.0 ** -12
+    xq, wq = (ops.mx_quantize(t.to(cuda_device), "nvfp4") for t in (x, w))
+    xv, wv = xq.dequantize(torch.float32).double(), wq.dequantize(torch.float32).double()
+    b = torch.zeros(n, device=cuda_device)
+    y, e = _product64(xv, wv, b.double(), None)
+    got = ops.mx_linear(xq, wq, b, out_dtype=torch.float32).double()
+    fits = y.abs() < torch.finfo(torch.float32).max / 2
+    assert fits[1].all() and fits[:, 5].all() == (sx * sw < 1e40)
+    # nvfp4 values are rounded once to fp32 above; half the smallest subnormal
+    assert ((got - y).abs() <= e + 2.0 ** -22 * y.abs() + 2.0 ** -149)[fits].all() and (got[1] == 0).all()
+    assert torch.isinf(got[y.abs() > e + 2.0 * torch.finfo(torch.float32).max]).all()
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("m", [1, 5, 48, 150, 600])
 def test_linear_without_bias_repeats_bitwise(cuda_device, fmt, m):
