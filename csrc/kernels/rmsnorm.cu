@@ -491,17 +491,11 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
             }
         }
         if (!here) {
-            abort = 1;
+            abort = j + 1;
             atomicCAS(a.status, 0, 4);
         }
         sum = group_sum<kThreads>(sum, red[j & 1]);
-        if (abort) {                             // (seen by all after the barrier in group_sum)
-            if (t == 0) {
-                const unsigned long long deadline = tc::drain_deadline();
-                for (int i = j; i < min(count, j + stages - 1); ++i) tc::mbar_drain(&full[i % stages], (i / stages) & 1, deadline);
-            }
-            break;
-        }
+        if (abort) break;                        // (seen by all after the barrier in group_sum)
         if (t == 0 && j + stages - 1 < count) load(j + stages - 1);
         const float c = sum * inv_dim * rstd * rstd * rstd;
 #pragma unroll
@@ -529,6 +523,10 @@ __global__ void __launch_bounds__(kThreads) rms_bwd_ring_kernel(RmsBwdArgs a, in
                 v.store(static_cast<T*>(a.gx) + r * a.dim, i, a.dim);
             }
         }
+    }
+    if (abort && t == 0) {      // rows that are still on their way, from the one that did not come
+        const unsigned long long deadline = tc::drain_deadline();
+        for (int j = abort - 1; j < min(count, abort + stages - 2); ++j) tc::mbar_drain(&full[j % stages], (j / stages) & 1, deadline);
     }
     if (!a.partial) return;
     float* dst = a.partial + static_cast<int64_t>(blockIdx.x) * rms_partial_pitch(a.dim);

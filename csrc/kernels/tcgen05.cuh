@@ -42,9 +42,10 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 // Bounded wait; false on timeout or when another role has aborted.
+template <typename Limit = long long>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const volatile int* abort,
-                                          long long limit = kWaitLimit) {
-    for (long long i = 0; i < limit; ++i) {
+                                          Limit limit = kWaitLimit) {
+    for (Limit i = 0; i < limit; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((i & 255) == 255 && *abort) return false;
     }
