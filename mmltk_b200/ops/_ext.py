@@ -63,6 +63,10 @@ def kernel_module_name() -> str:
 
 def kernels():
     """The CUDA kernel extension; raises if it is not built."""
+    if _environ is not None:      # (the short way of what follows)
+        loaded = _cache.get("_kernels_dbg" if _environ.get(b"MMLTK_DEBUG_BOUNDS") == b"1" else "_kernels")
+        if loaded is not None and loaded[0] is not None:
+            return loaded[0]
     mod, err = _load(kernel_module_name())
     if mod is None:
         raise RuntimeError(

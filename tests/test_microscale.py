@@ -236,7 +236,8 @@ def test_debug_switch_is_looked_up_at_every_call(monkeypatch):
 
         def __getattr__(self, name):
             raise AssertionError(name)
-    monkeypatch.setattr(_ext, "_load", lambda name: (Fake(name), None))
+    monkeypatch.setattr(_ext, "_cache", {})
+    monkeypatch.setattr(_ext, "_load", lambda name: _ext._cache.setdefault(name, (Fake(name), None)))
     x = OnGpu()
     calls = {"mx_quantize": lambda: ops.mx_quantize(x, "mxfp4"), "rms_norm": lambda: ops.rms_norm(x, x),
              "rms_norm_quantized": lambda: ops.rms_norm_quantized(x, x), "mx_status": lambda: ops.mx_status(torch.device("cuda", 0))}
