@@ -99,30 +99,32 @@ __global__ void __launch_bounds__(kQThreads, sizeof(T) == 2 ? 4 : 2)
     }
 }
 
-// Largest finite magnitude of kVecs vectors, as bits.  Infinities and NaN have bits above every number's: only where the
-// plain maximum shows one are the elements looked at again one by one.
-template <typename T, int kVecs>
-__device__ __forceinline__ uint32_t finite_amax_bits(const uint4* w) {
-    constexpr int kN = VecOf<T>::kN;
-    constexpr uint32_t kInf = 0x7f800000u;
-    uint32_t m = 0;
-    float f[kN];
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-        unpack16(w[u], f, T());
-#pragma unroll
-        for (int e = 0; e < kN; ++e) m = max(m, abs_bits(f[e]));
+// Running largest finite magnitude.  A magnitude's bits plus the distance from infinity to the sign bit stay positive, in
+// order, for finite numbers and turn negative for infinities and NaN, which a signed maximum then passes over: one
+// instruction a word beside the mask.
+template <typename T>
+struct FiniteMax {
+    static constexpr bool kWide = sizeof(T) == 4;
+    static constexpr uint32_t kOne = kWide ? 0x00800000u : (std::is_same_v<T, __half> ? 0x0400u : 0x0080u);
+    static constexpr uint32_t kBias = kWide ? kOne : kOne | kOne << 16;
+    uint32_t m = kBias;
+    __device__ __forceinline__ void word(uint32_t w) {
+        if constexpr (kWide) m = static_cast<uint32_t>(__viaddmax_s32(static_cast<int>(w & 0x7fffffffu), static_cast<int>(kBias), static_cast<int>(m)));
+        else m = __viaddmax_s16x2(w & 0x7fff7fffu, kBias, m);
     }
-    if (m < kInf) return m;
-    m = 0;
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-        unpack16(w[u], f, T());
-#pragma unroll
-        for (int e = 0; e < kN; ++e) m = max(m, abs_bits(f[e]) < kInf ? abs_bits(f[e]) : 0u);
+    __device__ __forceinline__ void add(const uint4& w) {
+        word(w.x);
+        word(w.y);
+        word(w.z);
+        word(w.w);
     }
-    return m;
-}
+    __device__ __forceinline__ uint32_t bits() const {      // of the value as fp32
+        if constexpr (kWide) return m - kOne;
+        const uint32_t t = max(m & 0xffffu, m >> 16) - kOne;
+        if constexpr (std::is_same_v<T, __half>) return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(t))));
+        return t << 16;
+    }
+};
 
 // Largest finite magnitude of each CTA's part of a matrix, as bits (max does not depend on the order); the pass that
 // reads them takes the largest.  A dense matrix is read as one row.
@@ -131,8 +133,7 @@ __global__ void __launch_bounds__(kAmaxThreads) mx_amax_kernel(const T* __restri
                                                       uint32_t* __restrict__ amax) {
     constexpr int kN = VecOf<T>::kN;
     __shared__ uint32_t warp_max[kAmaxThreads / 32];
-    uint32_t m = 0;
-    allow_next();
+    FiniteMax<T> top;
     wait_previous();
     // CTAs side by side in a row, then over the rows
     const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
@@ -145,15 +146,16 @@ __global__ void __launch_bounds__(kAmaxThreads) mx_amax_kernel(const T* __restri
             uint4 w[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) w[u] = reinterpret_cast<const uint4*>(row)[i + u * step];
-            m = max(m, finite_amax_bits<T, 4>(w));
+#pragma unroll
+            for (int u = 0; u < 4; ++u) top.add(w[u]);
         }
         for (; i < total; i += step) {
             const int64_t left = dim - i * kN;
-            const uint4 w = load_any(row + i * kN, left < kN ? static_cast<int>(left) : kN);
-            m = max(m, finite_amax_bits<T, 1>(&w));
+            top.add(load_any(row + i * kN, left < kN ? static_cast<int>(left) : kN));
         }
     }
-    m = __reduce_max_sync(0xffffffffu, m);
+    allow_next();
+    uint32_t m = __reduce_max_sync(0xffffffffu, top.bits());
     if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
     __syncthreads();
     if (threadIdx.x >= 32) return;
