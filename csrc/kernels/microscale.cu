@@ -7,10 +7,13 @@
 // r + 96: the four loads are in flight together, held as loaded, and the four rows' scale bytes are
 // neighbours in their tile.  The tiles' rows are put together in shared memory and leave as whole
 // sectors; a tile built from byte stores of CTAs that run at different times would reach DRAM in parts.
-// Measured, 16384 x 8192 bf16: mxfp4 52 us (6.5 TB/s), nvfp4 54 us, with the tensor's scale found first 97 us,
-// mxfp8 60 us; back to bf16 64 us (5.3 TB/s).  fp32: mxfp4 89 us, nvfp4 93 (105 at three CTAs an SM, which spill),
-// mxfp8 97.  1536 x 384: 2.6 us, nvfp4 with its scale found 4.8.  Reading all but the end of x past L2 in the pass for
-// the scale (for the second pass to find more there) changed nothing: 97 and 97 us.
+// Measured, graph replays, 16384 x 8192 bf16: mxfp4 52 us (6.5 TB/s), nvfp4 54 us, with the tensor's scale found first
+// 97 us (105 where replays alternate between two inputs: the end of x then waits in L2 for the second pass only), mxfp8
+// 60 us; back to bf16 64 to 69 us (5.2 to 5.9 TB/s).  fp32: mxfp4 89 us, nvfp4 93 (105 at three CTAs an SM, which
+// spill), mxfp8 97.  1536 x 384: 2.6 us, nvfp4 with its scale found 5.3.  Rows that are no multiple of 16 bytes
+// (16384 x 8191): mxfp4 89 us, nvfp4 92 and 141, mxfp8 94; back 151 to 155 us: their loads and stores are cut at the
+// granules of memory, vector by vector.  Reading all but the end of x past L2 in the pass for the scale (for the second
+// pass to find more there) changed nothing: 97 and 97 us.
 #include "microscale.cuh"
 
 namespace mmltk {

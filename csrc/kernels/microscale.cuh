@@ -52,7 +52,7 @@ struct BlockScale {
 // Power-of-two scale: the smallest 2^p whose 2^p * (largest element) is not below amax, so no element
 // saturates.  amax = 1.M * 2^(E - 127) against 1.5 * 2^2 (e2m1) or 1.75 * 2^8 (e4m3), on the bits;
 // clamped at 2^-127.  A block with an infinity or NaN gets the NaN scale (0xff): its values read back NaN
-// whatever their codes (zero for its finite elements and its padding).
+// whatever their codes (zero for its finite elements and its padding; that of a NaN for the others).
 template <int kBits>
 __device__ __forceinline__ BlockScale pow2_scale(float amax) {
     const uint32_t u = __float_as_uint(amax);

@@ -12,8 +12,10 @@
 // memory; after a cluster barrier the CTAs add the slices in their order, each a part of the
 // outputs, reading the others' shared memory.  No atomics, no workspace: the same bits every run.
 //
-// Measured, one token: nvfp4 4096 x 4096 6.0 us (17 as a quantisation and 128-row tiles), mxfp8 8192 x 8192 14.3 us
-// (4.85 TB/s); what is left above the weight's 1.4 and 10.6 us is set-up, one load latency and two cluster barriers.
+// Measured, one token, graph replays: nvfp4 4096 x 4096 5.8 to 6.0 us (17 as a quantisation and 128-row tiles); mxfp8
+// 8192 x 8192 17.0 us (4.1 TB/s) with weights in turn, 14.8 with one, which stays in L2.  What is left above the weight's
+// 1.4 and 10.6 us is set-up, one load latency (the first load waits for the kernel in front), the partial sums' way
+// through shared memory and two cluster barriers.
 //
 // Waits are bounded; on a time-out the kernel sets the status word and leaves.
 #include "mx_mma.cuh"

@@ -30,9 +30,10 @@
 // Few tiles and a long reduction: the CTAs of a cluster each take a slice of it, leave their partial sums in
 // their (now free) stages, and after a cluster barrier each finishes a part of the columns, adding the slices in order.
 //
-// Measured (B200, CUDA-graph replays): 8192^3 mxfp8 370 us (2.9 PFLOP/s), mxfp4 197 us (5.6), nvfp4 222 us (5.0).  These
-// run at the power cap (1.35 to 1.55 GHz; a bf16 cuBLAS product there 1.1 PFLOP/s); the tensor pipe is busy
-// 74 % of the cycles (4096^3 mxfp8).  nvfp4 is slower than mxfp4 by its scale copies: 12 a stage take 132
+// Measured (B200, CUDA-graph replays, x quantised before), 8192^3: mxfp8 370 to 387 us (2.9 PFLOP/s), mxfp4 195 to 197 us
+// (5.6), nvfp4 222 to 234 us (4.8) in bursts of some milliseconds.  Over two seconds the power cap sets in: mxfp8 445 us
+// at 1.24 GHz (2.5), mxfp4 223 at 1.49 (4.9), nvfp4 255 at 1.51 (4.3); a bf16 cuBLAS product there 1.43 PFLOP/s at
+// 1.38 GHz.  The tensor pipe is busy 74 % of the cycles (4096^3 mxfp8).  nvfp4 is slower than mxfp4 by its scale copies: 12 a stage take 132
 // cycles beside the MMAs' 512, 6 take 52, 3 none.  Short products are bound by issue slots: at
 // 31200 x 2048 x 256 to mxfp8 (29 us; 66 MB out, 10 us) the epilogue's warps use 58 % of them, and the
 // scheduler keeps a ready warp going, so the issuing warp waits for the epilogue's bursts.
@@ -764,8 +765,8 @@ cudaError_t by_output(const MxGemmArgs& g, cudaStream_t st, int splits = 1) {
 
 template <MxFormat F>
 cudaError_t by_tile(const MxGemmArgs& g, cudaStream_t st) {
-    // Pairs where the reduction is long (8 stages) and the pairs get two tiles each: at 8192^3 they take 392 us where
-    // 128 x 256 tiles of single CTAs take 462 (mxfp8) and 224 against 318 (nvfp4); at K = 256 they lose (31200 x 2048:
+    // Pairs where the reduction is long (8 stages) and the pairs get two tiles each: at 8192^3, both timed in turn at the
+    // power cap, they take 392 us where 128 x 256 tiles of single CTAs take 462 (mxfp8) and 224 against 318 (nvfp4); at K = 256 they lose (31200 x 2048:
     // 45 us against 30), each tile's hand-overs crossing the pair.  Else the width whose waves cost less, a
     // 256-column tile counting 1.75 of a 128-column one (31200 x 2048 x 256: 33.4 and 30.0; 10400 x 1536 x 384: 18.3
     // and 19.6; 512 x 4096 x 4096: 9.9 and 13.6).

@@ -10,9 +10,11 @@
 // elements, a CTA of 128 to 512 threads beyond -- so every element is read once; statistics are
 // fp32.  A thread's elements are 16-byte vectors kGroup vectors apart, so the 2 to 8 threads of a
 // scale block are neighbours in a warp and find its maximum with at most three shuffles.
-// Measured, bf16 with a residual: forward 32768 x 4096 157 us (6.8 TB/s), to mxfp8 139 us (6.8 TB/s); backward
-// 166 us (6.5 TB/s); 16384 x 7001, whose rows start anywhere, 145 and 175 us (at the copy's rate 140 and
-// 123), its backward without a residual 162 (105).
+// Measured, bf16 with a residual, graph replays: forward 32768 x 4096 157 us (6.8 TB/s), to mxfp8 139 us (6.8 TB/s), to
+// mxfp4 136, to nvfp4 146; backward 160 us (6.7 TB/s); 16384 x 7001, whose rows start anywhere, 145 and 175 us (at the
+// copy's rate 140 and 123), its backward without a residual 160 (105).  Replays write over outputs that are still in L2 as
+// the last one left them, which saves some of their way to memory; single calls of 32768 x 4096 to mxfp8 with other
+// buffers in between take 154 to 162 us.
 #include "microscale.cuh"
 #include "tcgen05.cuh"
 
@@ -396,8 +398,8 @@ __global__ void __launch_bounds__(kGroup == 32 ? 256 : kGroup, kGroup == 32 ? 3 
 
 // The same for rows of more than a warp: the inputs come through a ring of rows in shared memory (bulk asynchronous
 // copies), so what is in flight does not depend on registers; a row's stage is loaded again after the next row's
-// sum, when every thread has left it.  bf16, us (TB/s; loads into registers): 16384 x 8192 171 (6.3; 197), 32768 x 4096
-// 166 (6.5; 198), 65536 x 1024 101 (5.3; 119): a row of 1024 leaves little work between its two barriers.
+// sum, when every thread has left it.  bf16, us (TB/s; loads into registers): 16384 x 8192 167 (6.4; 197), 32768 x 4096
+// 160 (6.7; 198), 65536 x 1024 97 (5.5; 119): a row of 1024 leaves little work between its two barriers.
 // Bytes of a ring's row: where rows start anywhere, room for the granules that they share with their neighbours.
 template <typename T>
 __host__ __device__ constexpr uint32_t ring_slot(int dim, bool aligned) {
